@@ -271,6 +271,118 @@ int32_t qtts_op_sample_noalloc(int32_t device, const float * logits, int32_t V, 
                                int32_t target_frames, int32_t frame, int32_t eos_id, int32_t suppress_start,
                                uint64_t seed, int32_t * token_out, void * stream);
 
+/* ---- Operators around an 8-bit key/value cache, on device tensors ---------
+ * (no counterpart in the reference, whose cache is F16 or F32 and contiguous,
+ * src/tts_transformer.cpp:731-837).  All pointers of this section are DEVICE
+ * pointers owned by the caller unless a comment says host; nothing is allocated,
+ * no call synchronises, all work goes to `stream` (NULL: the default stream) of
+ * `device`, and the calling thread's current device is left as it was.  They can
+ * be captured into a graph.  Return 1, or 0 for arguments that are refused
+ * (message: qtts_create_error(), per thread; nothing has been launched then).
+ * Types are ggml's numbers: 0 F32, 1 F16, 30 BF16. */
+
+/* Rotary positions of q [rows][q_heads][dim] and k [rows][k_heads][dim] (k NULL:
+ * q alone): the first `rot` dims of each head turn by pos[row] * freq[i] radians,
+ * pairs (i, i + rot/2) or, interleaved, (2i, 2i + 1); `factor` multiplies the
+ * rotated dims; the rest is copied.  freq [rot/2] F64 (qtts_rope_freqs fills one).
+ * The angle is formed and reduced in 64 bits.  Strides in elements; the dims of a
+ * head are contiguous.  An output may be its input (same strides). */
+typedef struct qtts_rope_args {
+    int32_t device, type;             /* 1 F16, 30 BF16, 0 F32 */
+    int32_t rows, q_heads, k_heads, dim, rot, interleaved;
+    float factor;
+    const int32_t * pos;              /* [rows] */
+    const double * freq;              /* [rot/2] */
+    const void * q, * k;
+    void * q_out, * k_out;
+    int64_t q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
+} qtts_rope_args;
+int32_t qtts_op_rope(const qtts_rope_args * a, void * stream);
+/* Host: the angles per position of `rot` dims at base theta into freq [rot/2]
+ * (host memory), and the factor on the rotated values.  scaling 0 none; 1 linear:
+ * positions divided by `factor`; 2 NTK: theta * factor^(rot/(rot-2)); 3 YaRN:
+ * dims that turn more than beta_fast times over original_len positions stay,
+ * those below beta_slow are divided by `factor`, a ramp between, and values are
+ * multiplied by 0.1 ln(factor) + 1. */
+int32_t qtts_rope_freqs(int32_t scaling, int32_t rot, double theta, double factor, double original_len, double beta_fast,
+                        double beta_slow, double * freq, float * value_factor);
+
+/* An 8-bit paged cache over the caller's memory.  A page holds 64 tokens: 8-bit
+ * codes of K and V rows for every kv head and one F32 scale per block of 16
+ * tokens and head (value = code * scale; scale = largest magnitude / 127 or / 448,
+ * codes rounded to nearest even).  k_open / v_open hold the rows of a sequence's
+ * last two blocks in 16 bits (row of position p at p % 32), so a block is always
+ * quantised from 16-bit rows, its bits do not depend on how the rows arrived, and
+ * up to 16 rows may be taken back by a smaller length.  A block with a value that
+ * is not finite reads back as NaN.  Kernels check every page number, length and
+ * row range of the device arrays against these sizes: what does not fit is left
+ * out and sets a bit of *status (1 page, 2 length, 4 rows, 8 a page of dst_table
+ * that is in use), which the caller may read and clear when it likes. */
+typedef struct qtts_kv8 {
+    int32_t device;
+    int32_t code;                     /* 0 int8, 1 e4m3 */
+    int32_t row_type;                 /* 16-bit type of the rows: 1 F16, 30 BF16 */
+    int32_t n_kv_heads, head_dim;     /* head_dim 64, 128 or 256 */
+    int32_t n_pages;                  /* pages in the pool */
+    int32_t n_seqs;                   /* sequences: rows of the page table, lengths, rings */
+    int32_t max_pages;                /* columns of the page table */
+    void * k, * v;                    /* [n_pages][n_kv_heads][64][head_dim] codes */
+    float * k_scale, * v_scale;       /* [n_pages][n_kv_heads][4] */
+    void * k_open, * v_open;          /* [n_seqs][n_kv_heads][32][head_dim] of row_type */
+    int32_t * status;                 /* [1] or NULL */
+} qtts_kv8;
+/* Host: the status bits that a call with these HOST copies of table
+ * [n_seqs][max_pages], lens [n_seqs] and cu [n_seqs+1] (or NULL) would set; -1 on
+ * bad arguments.  For callers that want to check a plan before they upload it. */
+int32_t qtts_kv8_check(const qtts_kv8 * c, const int32_t * table, const int32_t * lens, const int32_t * cu, int32_t n_rows,
+                       int32_t max_new);
+/* Append: sequence b's rows cu[b] .. cu[b+1]-1 of k, v [n_rows][n_kv_heads][head_dim]
+ * (cu NULL: one row each) become its last ones; lens are the lengths AFTER the
+ * append.  max_new >= the most rows of one sequence.  Strides in elements. */
+int32_t qtts_op_kv8_append(const qtts_kv8 * c, const int32_t * table, const int32_t * lens, const int32_t * cu,
+                           const void * k, const void * v, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
+                           int32_t n_rows, int32_t max_new, void * stream);
+/* Read back: rows begin[b] .. (begin NULL: 0) of each sequence, cu[b+1]-cu[b] of
+ * them, as values of out_type into k, v [n_rows][n_kv_heads][head_dim]. */
+int32_t qtts_op_kv8_read(const qtts_kv8 * c, const int32_t * table, const int32_t * begin, const int32_t * cu,
+                         int32_t out_type, void * k, void * v, int32_t n_rows, int32_t max_rows, void * stream);
+/* Attention of q [n_rows][n_heads][head_dim] (row_type) over the cache: sequence b
+ * brings rows cu[b] .. cu[b+1]-1 (cu NULL: one each), the last of them at position
+ * lens[b]-1; row at position p sees keys j <= p and, with window > 0, j > p - window.
+ * A row that sees nothing gives zeros (lse -inf); rows of `out` that belong to no
+ * sequence stay as they were.  lse [n_rows][n_heads] F32 or NULL.  weight_in /
+ * weight_out [n_seqs][n_kv_heads] at weight_stride (both NULL: none; they may be
+ * the same): weight_out[b][h][j] = weight_in[b][h][j] + the softmax weights of key
+ * j over the head group and the rows, for j < lens[b].  ws: workspace of at least
+ * qtts_kv8_attend_ws() bytes, 16-byte aligned, that no other call in flight uses. */
+typedef struct qtts_kv8_attend {
+    const int32_t * table, * lens, * cu;
+    const void * q;
+    void * out;
+    int64_t q_row, q_head, o_row, o_head;
+    int32_t n_rows, max_q, n_heads, window;
+    float scale;
+    float * lse;
+    const float * weight_in;
+    float * weight_out;
+    int64_t weight_stride;
+    void * ws;
+    int64_t ws_bytes;
+} qtts_kv8_attend;
+int64_t qtts_kv8_attend_ws(const qtts_kv8 * c, const qtts_kv8_attend * a);
+int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * a, void * stream);
+/* Eviction: a sequence longer than budget keeps, for each kv head, its first
+ * `sinks` and last `recent` rows and the heaviest of the others by weight
+ * [n_seqs][n_kv_heads] at weight_stride (ties to the lower position, NaN counts as
+ * the heaviest), in order; others keep all.  The kept rows move to the pages of
+ * dst_table [n_seqs][dst_pages], which no sequence may use, requantised per block
+ * from their codes (a block that moves whole keeps its values).  lens_out
+ * [n_seqs], keep [n_seqs][n_kv_heads][budget] (-1 past the end), weight_out the
+ * same shape (0 past the end).  budget is a multiple of 16. */
+int32_t qtts_op_kv8_evict(const qtts_kv8 * c, const int32_t * table, const int32_t * lens, const int32_t * dst_table,
+                          int32_t dst_pages, const float * weight, int64_t weight_stride, int32_t budget, int32_t sinks,
+                          int32_t recent, int32_t * lens_out, int32_t * keep, float * weight_out, void * stream);
+
 /* ---- batched frame loop (B independent utterances on one GPU; no reference
  * counterpart: the reference serves one sequence per TTSTransformer).
  * Every projection of an F16 model is a tcgen05 tensor-core GEMM over the batch rows, the

@@ -13,7 +13,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libqwen3tts_b200.so")
-SOURCES = [os.path.join(HERE, "csrc", "engine.cu"), os.path.join(HERE, "csrc", "tts_transformer.cpp")]
+SOURCES = [os.path.join(HERE, "csrc", f) for f in ("engine.cu", "kv8.cu", "tts_transformer.cpp")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include")]
 

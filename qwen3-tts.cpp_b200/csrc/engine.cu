@@ -287,6 +287,7 @@ struct Engine {
 };
 
 static thread_local std::string g_create_error;
+void set_op_error(const char * msg) { g_create_error = msg; }   // device-tensor operators (kv8.cu)
 
 void Engine::build_rope(std::vector<float2> & t, int n_pos, float base) {
     // ggml_rope_cache_init (ext_factor 0, freq_scale 1, attn_factor 1): theta for
