@@ -115,6 +115,46 @@ template <class F> void by_cache(const qtts_kv8 & c, F f) {
     else by_code(__nv_bfloat16{});
 }
 
+// How an attention call runs.  Rows of a (sequence, kv head) come in tiles of 8 nt;
+// one CTA takes a tile's whole range, or, with few tiles over a long cache, the
+// ranges are split evenly over the GPU.
+struct K8Plan { int nt, tiles, split, ctas; int64_t part_bytes; unsigned grid; };
+constexpr int SMS = 148, SPLIT_CTAS = SMS * 4;
+bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
+    const int64_t R = (int64_t) p.max_q * (p.n_heads / c.n_kv_heads);
+    o->nt = R <= 8 ? 1 : (R <= 16 || c.head_dim == 256 ? 2 : 4);
+    const int64_t tiles = (R + 8 * o->nt - 1) / (8 * o->nt), items = tiles * c.n_kv_heads * c.n_seqs;
+    if (items > 0x7fffffff) return false;
+    o->tiles = (int) tiles;
+    o->split = c.max_pages > 8 && R <= 64 && c.n_seqs <= K8_MAX_SPLIT_SEQS;
+    o->ctas = SPLIT_CTAS;
+    o->part_bytes = o->split ? (int64_t) o->ctas * 2 * 8 * o->nt * (c.head_dim + 2) * 4 : 0;
+    o->grid = (unsigned)(o->split ? o->ctas : items);
+    return true;
+}
+template <class T, bool E4M3, int D, int NT>
+cudaError_t attend_launch(const K8AttendArgs & a, const K8Plan & p, cudaStream_t st) {
+    constexpr int NW = 4, join = k8_join_bytes<D, NT, NW>();
+    if (!p.split) {
+        auto f = k_kv8_attend_whole<T, E4M3, D, NT, NW>;
+        if (join > 48 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, join);
+            if (e != cudaSuccess) return e;
+        }
+        f<<<p.grid, NW * 32, join, st>>>(a);
+        return cudaGetLastError();
+    }
+    auto f = k_kv8_attend_split<T, E4M3, D, NT, NW>;
+    const int smem = join + (a.c.n_seqs + 1) * 8;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, join + (K8_MAX_SPLIT_SEQS + 1) * 8);
+        if (e != cudaSuccess) return e;
+    }
+    f<<<p.grid, NW * 32, smem, st>>>(a);
+    k_kv8_join<T, D, NT><<<(unsigned)(a.c.n_seqs * a.c.n_kv_heads), 128, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
 }  // namespace
 }  // namespace qtts
 
@@ -253,7 +293,9 @@ int32_t qtts_op_kv8_read(const qtts_kv8 * c, const int32_t * table, const int32_
 
 int64_t qtts_kv8_attend_ws(const qtts_kv8 * c, const qtts_kv8_attend * p) {
     if (bad_cache(c) || !p || p->n_rows < 0 || p->n_heads < 1) return -1;
-    return p->weight_out ? ((int64_t) p->n_rows * p->n_heads * 4 + 15) / 16 * 16 : 0;
+    K8Plan plan;
+    if (p->n_heads % c->n_kv_heads || p->max_q < 0 || !attend_plan(*c, *p, &plan)) return -1;
+    return plan.part_bytes + (p->weight_out && !p->lse ? ((int64_t) p->n_rows * p->n_heads * 4 + 15) / 16 * 16 : 0);
 }
 
 int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * p, void * stream) {
@@ -279,19 +321,27 @@ int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * p, void *
     a.q_row = p->q_row; a.q_head = p->q_head; a.o_row = p->o_row; a.o_head = p->o_head;
     a.n_rows = p->n_rows; a.max_q = p->max_q; a.n_heads = p->n_heads; a.window = p->window; a.scale = p->scale; a.lse = p->lse;
     a.w_in = p->weight_in; a.w_out = p->weight_out; a.w_stride = p->weight_stride;
-    unsigned g, gw = 0;
-    if (!grid_of((int64_t) c->n_seqs * p->max_q * p->n_heads, 4, &g) ||
-        (p->weight_out && !grid_of((int64_t) c->n_seqs * c->n_kv_heads * c->max_pages * K8_PAGE, 4, &gw)))
-        return refuse(who, "too much work for one call");
-    float * lse_ws = p->weight_out ? static_cast<float *>(p->ws) : nullptr;
+    unsigned gw = 0;
+    if (p->weight_out && !grid_of((int64_t) c->n_seqs * c->n_kv_heads * c->max_pages * K8_PAGE, 4, &gw)) return refuse(who, "too much work for one call");
+    K8Plan plan;
+    if (!attend_plan(*c, *p, &plan)) return refuse(who, "too much work for one call");
+    if (p->weight_out && !a.lse) a.lse = reinterpret_cast<float *>(static_cast<uint8_t *>(p->ws) + plan.part_bytes);
+    a.part = static_cast<float *>(p->ws);
+    a.tiles = plan.tiles; a.ctas = plan.ctas;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t err = cudaSuccess;
     by_cache(*c, [&](auto t, auto e, auto d) {
         using T = decltype(t);
         constexpr bool E = decltype(e)::value;
         constexpr int D = decltype(d)::value;
-        if (g) k_kv8_attend_plain<T, E, D><<<g, 128, 0, st>>>(a, lse_ws);
-        if (p->weight_out) k_kv8_weigh_plain<T, E, D><<<gw, 128, 0, st>>>(a, lse_ws);
+        if (p->n_rows > 0 && p->max_q > 0) {
+            if (plan.nt == 1) err = attend_launch<T, E, D, 1>(a, plan, st);
+            else if (plan.nt == 2) err = attend_launch<T, E, D, 2>(a, plan, st);
+            else if constexpr (D < 256) err = attend_launch<T, E, D, 4>(a, plan, st);
+        }
+        if (p->weight_out) k_kv8_weigh_plain<T, E, D><<<gw, 128, 0, st>>>(a, a.lse);
     });
+    if (err != cudaSuccess) return refuse(who, cudaGetErrorString(err));
     return launched(who);
 }
 

@@ -6,6 +6,9 @@
 // over the keys j that a row sees: j <= p and, with a window w, j > p - w, where
 // p = len - n + i is the position of row i of the n rows that a sequence brings.
 // A row that sees nothing gives zeros and lse = -inf.
+//
+// The products run on the tensor cores in F16 with F32 sums: codes of both kinds
+// are exact in F16, the scales stay outside in F32.
 #pragma once
 #include "kv8.cuh"
 
@@ -23,6 +26,9 @@ struct K8AttendArgs {
     const float * w_in;                        // [n_seqs][H][w_stride] or null
     float * w_out;
     int64_t w_stride;
+    float * part;                              // partial results (split kernel), see K8Split
+    int tiles;                                 // row tiles of one (sequence, kv head)
+    int ctas;                                  // CTAs of the split kernel
 };
 
 // Keys [lo, hi) of row i of a sequence.
@@ -32,51 +38,496 @@ __device__ __forceinline__ void k8_span(const K8Seq & s, int i, int window, int 
     lo = window > 0 && p - window + 1 > 0 ? p - window + 1 : 0;
 }
 
-// The plain kernel: one warp per (row, query head), a lane owns D / 32 dims, one
-// key at a time with the running maximum and sum.  Right for every case; bound by
-// the five shuffles of each key.
-template <class T, bool E4M3, int D>
-__global__ void __launch_bounds__(128) k_kv8_attend_plain(K8AttendArgs a, float * lse_ws) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31, H = a.c.n_kv_heads, G = a.n_heads / H;
-    const int64_t unit = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int hq = (int)(unit % a.n_heads), i = (int)(unit / a.n_heads % a.max_q);
-    const int64_t b = unit / a.n_heads / a.max_q;
-    if (b >= a.c.n_seqs) return;
-    const K8Seq s = k8_seq((int) b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
-    if (s.status && lane == 0) k8_flag(a.c.status, s.status);
-    if (i >= s.n) return;
-    const int h = hq / G, row = s.row0 + i;
-    int lo, hi;
-    k8_span(s, i, a.window, lo, hi);
-    const T * q = static_cast<const T *>(a.q) + row * a.q_row + hq * a.q_head + lane * V;
-    float qv[V], o[V];
+// ---- fragments ---------------------------------------------------------------
+// The scores are formed transposed, S^T = K Q^T (16 keys x 8 rows per MMA), and so
+// is the output, O^T = V^T P^T (16 dims x 8 rows): with one query token a group of
+// G <= 8 heads fills one MMA column tile, where the usual orientation would pad it
+// to 16.  An MMA's inner index may be permuted freely if both operands agree, so a
+// lane loads what it needs straight from the page as 16-byte words:
+//   K: lane (g, t) = (lane / 4, lane % 4) holds 16 consecutive dims of keys g and g + 8
+//      per 64 dims; word w of them is one k-step (4 dims a lane).
+//   V: the lane holds D / 8 dims (from 16 g on, per 128) of tokens 2t, 2t+1, 2t+8, 2t+9;
+//      dims 2j and 2j+1 of them are rows g and g + 8 of output tile j.
+// No shared memory or transposition is needed between the page and the MMA.
+__device__ __forceinline__ uint32_t k8_prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
+// Four codes -> two F16 pairs (bytes 0, 1 and 2, 3).
+template <bool E4M3> __device__ __forceinline__ void k8_f16x4(uint32_t w, uint32_t & lo, uint32_t & hi);
+template <> __device__ __forceinline__ void k8_f16x4<false>(uint32_t w, uint32_t & lo, uint32_t & hi) {
+    // byte u = code + 128 as the low mantissa bits of 1024: 1024 + u - 1152 = code, exactly
+    w ^= 0x80808080u;
+    lo = k8_prmt(w, 0x64646464u, 0x4140);
+    hi = k8_prmt(w, 0x64646464u, 0x4342);
+    const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    __half2 a = __hsub2(*reinterpret_cast<__half2 *>(&lo), off), b = __hsub2(*reinterpret_cast<__half2 *>(&hi), off);
+    lo = *reinterpret_cast<uint32_t *>(&a);
+    hi = *reinterpret_cast<uint32_t *>(&b);
+}
+template <> __device__ __forceinline__ void k8_f16x4<true>(uint32_t w, uint32_t & lo, uint32_t & hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ void k8_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float k8_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t k8_pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t k8_transpose(uint32_t x) {   // an 8 x 8 matrix of 16-bit values over the warp
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 k8_ld16(const uint8_t * p) { return ld_stream(p); }
+__device__ __forceinline__ uint2 k8_ld8b(const uint8_t * p) {
+    uint2 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+    return r;
+}
+
+// One block's K words of a lane: keys g and g + 8, D / 16 words each.
+template <int D> struct K8K { uint32_t a[D / 16], b[D / 16]; };
+template <int D> __device__ __forceinline__ void k8_load_k(K8K<D> & k, const uint8_t * base, int lane) {
+    const uint8_t * p = base + (lane >> 2) * D + (lane & 3) * 16;
 #pragma unroll
-    for (int e = 0; e < V; ++e) { qv[e] = (float) q[e]; o[e] = 0.0f; }
-    float m = -INFINITY, l = 0.0f;
-    for (int j = lo; j < hi; ++j) {
-        const int page = k8_page(a.table + b * a.c.max_pages, j / K8_PAGE, a.c.n_pages);
-        if (page < 0) { if (lane == 0) k8_flag(a.c.status, K8_BAD_PAGE); continue; }
-        const int64_t at = k8_code_off(page, h, j % K8_PAGE, H, D) + lane * V, sa = k8_scale_off(page, h, j % K8_PAGE / K8_BLOCK, H);
-        float d = 0.0f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) d = fmaf(qv[e], Code8<E4M3>::value(static_cast<const uint8_t *>(a.c.k)[at + e]), d);
-        d = warp_sum(d) * a.c.k_scale[sa] * a.scale;
-        const float m2 = fmaxf(m, d);
-        const float f = expf(m - m2), p = expf(d - m2), ps = p * a.c.v_scale[sa];
-        l = l * f + p;
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = fmaf(ps, Code8<E4M3>::value(static_cast<const uint8_t *>(a.c.v)[at + e]), o[e] * f);
-        m = m2;
+    for (int c = 0; c < D / 64; ++c) {
+        const uint4 x = k8_ld16(p + c * 64), y = k8_ld16(p + 8 * D + c * 64);
+        k.a[4 * c] = x.x; k.a[4 * c + 1] = x.y; k.a[4 * c + 2] = x.z; k.a[4 * c + 3] = x.w;
+        k.b[4 * c] = y.x; k.b[4 * c + 1] = y.y; k.b[4 * c + 2] = y.z; k.b[4 * c + 3] = y.w;
     }
-    T * out = static_cast<T *>(a.out) + row * a.o_row + hq * a.o_head + lane * V;
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+}
+// One block's V words: tokens 2t, 2t+1, 2t+8, 2t+9, D / 32 words each.
+template <int D> struct K8V { uint32_t w[4][D / 32]; };
+template <int D> __device__ __forceinline__ void k8_load_v(K8V<D> & v, const uint8_t * base, int lane) {
+    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = T(l == 0.0f ? 0.0f : o[e] * inv);
-    if (lane == 0) {
-        const float L = l == 0.0f ? -INFINITY : m + logf(l);
-        if (a.lse) a.lse[(int64_t) row * a.n_heads + hq] = L;
-        if (lse_ws) lse_ws[(int64_t) row * a.n_heads + hq] = L;
+    for (int i = 0; i < 4; ++i) {
+        const uint8_t * p = base + (2 * t + (i & 1) + (i >> 1) * 8) * D;
+        if constexpr (D == 64) {
+            const uint2 x = k8_ld8b(p + g * 8);
+            v.w[i][0] = x.x; v.w[i][1] = x.y;
+        } else {
+#pragma unroll
+            for (int c = 0; c < D / 128; ++c) {
+                const uint4 x = k8_ld16(p + c * 128 + g * 16);
+                v.w[i][4 * c] = x.x; v.w[i][4 * c + 1] = x.y; v.w[i][4 * c + 2] = x.z; v.w[i][4 * c + 3] = x.w;
+            }
+        }
+    }
+}
+// The first dim of output tile j of a lane (its second one follows).
+template <int D> __device__ __forceinline__ int k8_dim(int j, int lane) {
+    const int g = lane >> 2;
+    if constexpr (D == 64) return g * 8 + 2 * j;
+    else return (j >> 3) * 128 + g * 16 + 2 * (j & 7);
+}
+
+// The query rows of a tile as MMA column fragments: row g (+ 8 nt) of a lane, dims as
+// in K.  BF16 rows are scaled by a power of two to a largest magnitude in [1, 2)
+// first (F16 has their precision but not their range; what falls below F16's
+// smallest step is 2^-25 of the row's largest value); `back` undoes it.
+template <class T, int D> struct K8Q { uint32_t x[D / 16][2]; };
+template <class T, int D>
+__device__ __forceinline__ float k8_load_q(K8Q<T, D> & q, const T * row, int lane, bool real) {
+    const uint16_t * p = reinterpret_cast<const uint16_t *>(row) + (lane & 3) * 16;
+    uint32_t most = 0;
+    const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+        uint32_t w[8];
+        if (!real) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = 0;
+        } else if (vec) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(p + c * 64), y = *reinterpret_cast<const uint4 *>(p + c * 64 + 8);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = p[c * 64 + 2 * i] | (uint32_t) p[c * 64 + 2 * i + 1] << 16;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            q.x[4 * c + (i >> 1)][i & 1] = w[i];
+            most = max(most, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+        }
+    }
+    if constexpr (sizeof(T) == 2 && Row16<T>::inf == 0x7c00u) return 1.0f;
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // 2^-e and 2^e of the largest magnitude's exponent, kept within F32
+    int e = (int)(most >> 7) - 127;
+    e = most == 0 || most >= Row16<T>::inf ? 0 : max(-120, min(120, e));
+    const float down = __int_as_float((127 - e) << 23), back = __int_as_float((127 + e) << 23);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t w = q.x[i][j];
+            q.x[i][j] = k8_pack(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
+        }
+    return back;
+}
+
+// ---- few rows ----------------------------------------------------------------
+// One warp's running state over its blocks: reference value m (log2 units) and sum
+// per row, unnormalised output.  The reference moves only when a score passes it by
+// more than 4 (a vote), so most blocks need no reduction over lanes; weights are
+// 2^(s - m + 8), at most 2^12 and in F16's normal range down to 2^-22 of the
+// largest.  They are rounded to F16 for the product with V (half a step is 2^-12
+// relative, independent from key to key, under the output's own rounding); their
+// sum is taken before that, in F32.
+constexpr float K8_LIFT = 8.0f, K8_SLACK = 4.0f;
+template <int D, int NT> struct K8State {
+    float m[NT][2], l[NT][2], o[NT][D / 16][4];   // rows 8 nt + 2t, + 1
+};
+
+// Segment of one warp: blocks first, first + step, .. < last of a sequence.
+struct K8Rows { int lo[2], hi[2]; };              // keys of the lane's rows 8 nt + 2t + {0, 1}
+
+template <bool E4M3, class T, int D, int NT>
+__device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (&q)[NT], const float (&fac)[NT][2], const K8Rows (&rows)[NT],
+                                          const K8AttendArgs & a, const int32_t * table, int h, int first, int last, int step, int all_lo, int all_hi,
+                                          int any_hi, int lane) {
+    const int H = a.c.n_kv_heads;
+    const uint8_t * kc = static_cast<const uint8_t *>(a.c.k), * vc = static_cast<const uint8_t *>(a.c.v);
+    if (first >= last) return;
+    K8K<D> k;
+    K8V<D> v;
+    float ks = 0.0f, vs = 0.0f;
+    int page = k8_page(table, first / K8_BPP, a.c.n_pages);
+    int next = first + step < last ? k8_page(table, (first + step) / K8_BPP, a.c.n_pages) : -1;
+    auto off = [&](int pg, int X) { return k8_code_off(pg, h, X % K8_BPP * K8_BLOCK, H, D); };
+    if (page >= 0) {
+        k8_load_k<D>(k, kc + off(page, first), lane);
+        k8_load_v<D>(v, vc + off(page, first), lane);
+        ks = a.c.k_scale[k8_scale_off(page, h, first % K8_BPP, H)];
+        vs = a.c.v_scale[k8_scale_off(page, h, first % K8_BPP, H)];
+    }
+    for (int X = first; X < last; X += step) {
+        const int nX = X + step;
+        const int nnext = nX + step < last ? k8_page(table, (nX + step) / K8_BPP, a.c.n_pages) : -1;
+        const float ks0 = ks, vs0 = vs;
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            uint32_t a0, a1, a2, a3;
+            k8_f16x4<E4M3>(k.a[i], a0, a2);
+            k8_f16x4<E4M3>(k.b[i], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) k8_mma(s[nt], a0, a1, a2, a3, q[nt].x[i][0], q[nt].x[i][1]);
+        }
+        const bool have = page >= 0;
+        if (!have && lane == 0) k8_flag(a.c.status, K8_BAD_PAGE);
+        if (nX < last && next >= 0) {
+            k8_load_k<D>(k, kc + off(next, nX), lane);
+            ks = a.c.k_scale[k8_scale_off(next, h, nX % K8_BPP, H)];
+            vs = a.c.v_scale[k8_scale_off(next, h, nX % K8_BPP, H)];
+        }
+        if (have) {
+            const bool whole = X * K8_BLOCK >= all_lo && X * K8_BLOCK + K8_BLOCK <= all_hi;   // every row sees every key
+            bool up = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[nt][e] *= fac[nt][e & 1] * ks0;
+                    if (!whole) {
+                        const int j = X * K8_BLOCK + (lane >> 2) + (e >> 1) * 8;
+                        if (j < rows[nt].lo[e & 1] || j >= rows[nt].hi[e & 1]) s[nt][e] = -INFINITY;
+                    }
+                }
+                up |= fmaxf(s[nt][0], s[nt][2]) > st.m[nt][0] + K8_SLACK || fmaxf(s[nt][1], s[nt][3]) > st.m[nt][1] + K8_SLACK;
+            }
+            if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float m = fmaxf(s[nt][r], s[nt][r + 2]);
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                        m = fmaxf(m, st.m[nt][r]);
+                        const float f = m == st.m[nt][r] ? 1.0f : k8_exp2(st.m[nt][r] - m);
+                        st.m[nt][r] = m;
+                        st.l[nt][r] *= f;
+#pragma unroll
+                        for (int j = 0; j < D / 16; ++j) { st.o[nt][j][r] *= f; st.o[nt][j][r + 2] *= f; }
+                    }
+            }
+            uint32_t p[NT][2];
+            float fv[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    e[i] = k8_exp2(s[nt][i] - st.m[nt][i & 1] + K8_LIFT);
+                    if (!whole && s[nt][i] == -INFINITY) e[i] = 0.0f;   // (-inf) - (-inf) of a row that has seen nothing yet
+                }
+                st.l[nt][0] += e[0] + e[2];
+                st.l[nt][1] += e[1] + e[3];
+                p[nt][0] = k8_transpose(k8_pack(e[0], e[1]));
+                p[nt][1] = k8_transpose(k8_pack(e[2], e[3]));
+#pragma unroll
+                for (int r = 0; r < 2; ++r)   // a block that a row does not see adds nothing, even if its scale is NaN
+                    fv[nt][r] = whole || (X * K8_BLOCK < rows[nt].hi[r] && X * K8_BLOCK + K8_BLOCK > rows[nt].lo[r]) ? vs0 : 0.0f;
+            }
+            if (!whole) {   // rows of the page past the sequence's end may hold anything
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (X * K8_BLOCK + 2 * (lane & 3) + (i & 1) + (i >> 1) * 8 >= any_hi)
+#pragma unroll
+                        for (int w = 0; w < D / 32; ++w) v.w[i][w] = 0;
+            }
+#pragma unroll
+            for (int w = 0; w < D / 32; ++w) {
+                uint32_t a0[2], a1[2], a2[2], a3[2];
+                // tokens' bytes side by side: [x0 y0 x1 y1], [x2 y2 x3 y3]
+                k8_f16x4<E4M3>(k8_prmt(v.w[0][w], v.w[1][w], 0x5140), a0[0], a1[0]);
+                k8_f16x4<E4M3>(k8_prmt(v.w[0][w], v.w[1][w], 0x7362), a0[1], a1[1]);
+                k8_f16x4<E4M3>(k8_prmt(v.w[2][w], v.w[3][w], 0x5140), a2[0], a3[0]);
+                k8_f16x4<E4M3>(k8_prmt(v.w[2][w], v.w[3][w], 0x7362), a2[1], a3[1]);
+#pragma unroll
+                for (int o = 0; o < 2; ++o)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        k8_mma(c, a0[o], a1[o], a2[o], a3[o], p[nt][0], p[nt][1]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) st.o[nt][2 * w + o][e] = fmaf(c[e], fv[nt][e & 1], st.o[nt][2 * w + o][e]);
+                    }
+            }
+        }
+        if (nX < last && next >= 0) k8_load_v<D>(v, vc + off(next, nX), lane);
+        page = next;
+        next = nnext;
+    }
+}
+
+// What a CTA of the split kernel leaves of an item it has only a part of:
+// [CTA][first or last segment][8 NT rows] of m, l and [8 NT rows][D] of o.
+template <int D, int NT> struct K8Part { static constexpr int floats = 8 * NT * (D + 2); };
+
+// Pages [pg0, pg1) of a sequence that any of its rows sees.
+__device__ __forceinline__ void k8_pages(const K8Seq & s, int window, int & pg0, int & pg1) {
+    int lo, hi;
+    k8_span(s, 0, window, lo, hi);
+    pg0 = lo / K8_PAGE;
+    pg1 = s.n > 0 ? (s.len + K8_PAGE - 1) / K8_PAGE : 0;
+    if (pg1 < pg0) pg1 = pg0;
+}
+
+template <class T> __device__ __forceinline__ void k8_write_row(const K8AttendArgs & a, int row, int hq, int d, float o, float inv) {
+    static_cast<T *>(a.out)[row * a.o_row + hq * a.o_head + d] = T(o * inv);
+}
+
+// One segment (pages of one (sequence, kv head, row tile)) by the whole CTA: the
+// warps take its 16-key blocks in turn, their states are joined in shared memory in
+// warp order.  `dst` null: the item is complete and goes to out and lse.
+template <class T, bool E4M3, int D, int NT, int NW>
+__device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq & s, int b, int h, int tile, int pg0, int pg1, float * dst, float * smem) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3;
+    const int G = a.n_heads / a.c.n_kv_heads, R = s.n * G, r0 = tile * 8 * NT;
+    K8Q<T, D> q[NT];
+    float fac[NT][2];
+    K8Rows rows[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = r0 + nt * 8 + (lane >> 2);
+        const bool real = r < R;
+        const T * src = static_cast<const T *>(a.q) + (real ? (s.row0 + r / G) * a.q_row + (h * G + r % G) * a.q_head : 0);
+        const float back = k8_load_q<T, D>(q[nt], src, lane, real) * (a.scale * 1.44269504088896340736f);   // log2 e
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            fac[nt][i] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * i);
+            const int rr = r0 + nt * 8 + 2 * t + i;
+            // rows of padding see what the last one sees, so that they force no masking
+            k8_span(s, min(rr, R - 1) / G, a.window, rows[nt].lo[i], rows[nt].hi[i]);
+        }
+    }
+    int lo, hi, lo1, hi1;
+    k8_span(s, r0 / G, a.window, lo, hi);
+    k8_span(s, min(r0 + 8 * NT - 1, R - 1) / G, a.window, lo1, hi1);
+    K8State<D, NT> st;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            st.m[nt][i] = -INFINITY;
+            st.l[nt][i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) st.o[nt][j][i] = st.o[nt][j][i + 2] = 0.0f;
+        }
+    const int X0 = max(pg0 * K8_BPP, lo / K8_BLOCK), X1 = min(pg1 * K8_BPP, (hi1 + K8_BLOCK - 1) / K8_BLOCK);
+    k8_blocks<E4M3, T, D, NT>(st, q, fac, rows, a, a.table + (int64_t) b * a.c.max_pages, h, X0 + warp, X1, NW, lo1, hi, hi1, lane);
+    // join: rows' sums over lanes, then the warps through shared memory
+    float * sm = smem, * sl = smem + NW * 8 * NT, * so = smem + 2 * NW * 8 * NT;   // [NW][8 NT] twice, [NW][8 NT][D + 4]
+    constexpr int LD = D + 4;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float l = st.l[nt][i];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const int r = nt * 8 + 2 * t + i;
+            if (lane < 4) { sm[warp * 8 * NT + r] = st.m[nt][i]; sl[warp * 8 * NT + r] = l; }
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+                *reinterpret_cast<float2 *>(so + (warp * 8 * NT + r) * LD + k8_dim<D>(j, lane)) = make_float2(st.o[nt][j][i], st.o[nt][j][i + 2]);
+        }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 8 * NT * D; e += NW * 32) {
+        const int r = e / D, d = e % D, rr = r0 + r;
+        if (rr >= R) break;
+        float m = -INFINITY, l = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, sm[w * 8 * NT + r]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float mw = sm[w * 8 * NT + r], f = mw == m ? 1.0f : k8_exp2(mw - m);
+            l = fmaf(sl[w * 8 * NT + r], f, l);
+            o = fmaf(so[(w * 8 * NT + r) * LD + d], f, o);
+        }
+        if (dst) {
+            if (d == 0) { dst[r] = m; dst[8 * NT + r] = l; }
+            dst[16 * NT + r * D + d] = o;
+        } else {
+            const int row = s.row0 + rr / G, hq = h * G + rr % G;
+            k8_write_row<T>(a, row, hq, d, o, l == 0.0f ? 0.0f : 1.0f / l);
+            if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = l == 0.0f ? -INFINITY : (m - K8_LIFT + log2f(l)) * 0.693147180559945309417f;
+        }
+    }
+    __syncthreads();
+}
+template <int D, int NT, int NW> __host__ __device__ constexpr int k8_join_bytes() { return (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4; }
+
+// One CTA per (sequence, kv head, row tile).
+template <class T, bool E4M3, int D, int NT, int NW>
+__global__ void __launch_bounds__(NW * 32) k_kv8_attend_whole(K8AttendArgs a) {
+    extern __shared__ __align__(16) float k8_smem[];
+    const int H = a.c.n_kv_heads, G = a.n_heads / H;
+    const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles % H, b = blockIdx.x / a.tiles / H;
+    const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
+    if (threadIdx.x == 0 && h == 0 && tile == 0) k8_flag(a.c.status, s.status);
+    if (tile * 8 * NT >= s.n * G) return;
+    int pg0, pg1;
+    k8_pages(s, a.window, pg0, pg1);
+    k8_segment<T, E4M3, D, NT, NW>(a, s, b, h, tile, pg0, pg1, nullptr, k8_smem);
+}
+
+// Split along the cache.  All (sequence, kv head, row tile) items laid end to end are
+// T pages of work; CTA c takes pages [c * chunk, (c + 1) * chunk) of that line, so
+// ragged lengths balance to a page whatever they are.  An item that a CTA holds
+// whole is finished there; parts (a CTA's first and last segment at most) go to
+// `part` and are joined by k_kv8_join.
+constexpr int K8_MAX_SPLIT_SEQS = 1024, K8_MIN_PAGES = 4;
+// Prefix sums over the sequences of their pages of work in `at` [n_seqs + 1].
+template <int NT, int THREADS>
+__device__ __forceinline__ void k8_line(const K8AttendArgs & a, long long * at, long long * s_carry) {
+    const int H = a.c.n_kv_heads, G = a.n_heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) { at[0] = 0; }
+    long long base = 0;
+    for (int b0 = 0; b0 < a.c.n_seqs; b0 += THREADS) {
+        const int b = b0 + threadIdx.x;
+        long long w = 0;
+        if (b < a.c.n_seqs) {
+            const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
+            if (blockIdx.x == 0) k8_flag(a.c.status, s.status);
+            int pg0, pg1;
+            k8_pages(s, a.window, pg0, pg1);
+            w = (long long)(pg1 - pg0) * H * ((s.n * G + 8 * NT - 1) / (8 * NT));
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, w, o); if (lane >= o) w += y; }
+        __syncthreads();
+        if (lane == 31) s_carry[warp] = w;
+        __syncthreads();
+        long long before = base;
+        for (int i = 0; i < warp; ++i) before += s_carry[i];
+        if (b < a.c.n_seqs) at[b + 1] = before + w;
+        for (int i = 0; i < THREADS / 32; ++i) base += s_carry[i];
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ long long k8_chunk(long long total, int ctas) {
+    const long long c = (total + ctas - 1) / ctas;
+    return c < K8_MIN_PAGES ? K8_MIN_PAGES : c;
+}
+
+template <class T, bool E4M3, int D, int NT, int NW>
+__global__ void __launch_bounds__(NW * 32) k_kv8_attend_split(K8AttendArgs a) {
+    extern __shared__ __align__(16) float k8_smem[];
+    __shared__ long long s_carry[NW];
+    long long * at = reinterpret_cast<long long *>(k8_smem + k8_join_bytes<D, NT, NW>() / 4);
+    k8_line<NT, NW * 32>(a, at, s_carry);
+    const long long total = at[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
+    long long pos = blockIdx.x * chunk;
+    const long long end = pos + chunk < total ? pos + chunk : total;
+    const int G = a.n_heads / a.c.n_kv_heads;
+    bool first = true;
+    while (pos < end) {
+        int lo = 0, hi = a.c.n_seqs - 1;            // the last sequence that begins at or before pos
+        while (lo < hi) { const int mid = (lo + hi + 1) / 2; if (at[mid] <= pos) lo = mid; else hi = mid - 1; }
+        const K8Seq s = k8_seq(lo, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
+        int pg0, pg1;
+        k8_pages(s, a.window, pg0, pg1);
+        const int np = pg1 - pg0, tiles = (s.n * G + 8 * NT - 1) / (8 * NT);
+        const long long in = pos - at[lo];
+        const int item = (int)(in / np), p0 = (int)(in % np);
+        const int p1 = (int)(np - p0 < end - pos ? np : p0 + (end - pos));
+        const bool whole = p0 == 0 && p1 == np;
+        float * dst = whole ? nullptr : a.part + ((long long) blockIdx.x * 2 + (first ? 0 : 1)) * K8Part<D, NT>::floats;
+        k8_segment<T, E4M3, D, NT, NW>(a, s, lo, item / tiles, item % tiles, pg0 + p0, pg0 + p1, dst, k8_smem);
+        pos += p1 - p0;
+        first = false;
+    }
+}
+
+// Joins the parts of an item in the order of the cache, one CTA per (sequence, kv head);
+// rows of items without pages become zeros.
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(128) k_kv8_join(K8AttendArgs a) {
+    __shared__ long long at[K8_MAX_SPLIT_SEQS + 1], s_carry[4];
+    const int H = a.c.n_kv_heads, G = a.n_heads / H, h = blockIdx.x % H, b = blockIdx.x / H;
+    k8_line<NT, 128>(a, at, s_carry);
+    const long long total = at[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
+    const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
+    int pg0, pg1;
+    k8_pages(s, a.window, pg0, pg1);
+    const int np = pg1 - pg0, tiles = (s.n * G + 8 * NT - 1) / (8 * NT);
+    for (int tile = 0; tile < tiles; ++tile) {
+        const long long p0 = at[b] + (long long)(h * tiles + tile) * np, p1 = p0 + np;
+        const int c0 = (int)(p0 / chunk), c1 = np ? (int)((p1 - 1) / chunk) : c0 - 1;
+        if (c0 == c1) continue;
+        for (int e = threadIdx.x; e < 8 * NT * D; e += 128) {
+            const int r = e / D, d = e % D, rr = tile * 8 * NT + r;
+            if (rr >= s.n * G) break;
+            float m = -INFINITY, l = 0.0f, o = 0.0f;
+            auto slot = [&](int c) { return a.part + ((long long) c * 2 + (c == c0 && p0 > c * chunk ? 1 : 0)) * K8Part<D, NT>::floats; };
+            for (int c = c0; c <= c1; ++c) m = fmaxf(m, slot(c)[r]);
+            for (int c = c0; c <= c1; ++c) {
+                const float * p = slot(c);
+                const float f = p[r] == m ? 1.0f : k8_exp2(p[r] - m);
+                l = fmaf(p[8 * NT + r], f, l);
+                o = fmaf(p[16 * NT + r * D + d], f, o);
+            }
+            const int row = s.row0 + rr / G, hq = h * G + rr % G;
+            k8_write_row<T>(a, row, hq, d, o, l == 0.0f ? 0.0f : 1.0f / l);
+            if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = l == 0.0f ? -INFINITY : (m - K8_LIFT + log2f(l)) * 0.693147180559945309417f;
+        }
     }
 }
 
