@@ -1,6 +1,7 @@
 // kv8.cu — C entry points of the rotary and 8-bit-cache operators: argument
 // checks, then launches on the caller's stream.  No entry allocates device memory
 // or throws.
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <string>
@@ -119,7 +120,12 @@ template <class F> void by_cache(const qtts_kv8 & c, F f) {
 // one CTA takes a tile's whole range, or, with few tiles over a long cache, the
 // ranges are split evenly over the GPU.
 struct K8Plan { int nt, tiles, split, ctas; int64_t part_bytes; unsigned grid; };
-constexpr int SMS = 148, SPLIT_CTAS = SMS * 4;
+constexpr int SMS = 148, NW = 4;
+// CTAs of the split kernel that are resident together (registers, then shared memory)
+int split_ctas(int dim, int nt) {
+    const int per = dim == 256 ? 2 : (nt == 1 ? 4 : (nt == 2 ? 3 : 2));
+    return SMS * per;
+}
 bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     const int64_t R = (int64_t) p.max_q * (p.n_heads / c.n_kv_heads);
     o->nt = R <= 8 ? 1 : (R <= 16 || c.head_dim == 256 ? 2 : 4);
@@ -127,32 +133,47 @@ bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     if (items > 0x7fffffff) return false;
     o->tiles = (int) tiles;
     o->split = c.max_pages > 8 && R <= 64 && c.n_seqs <= K8_MAX_SPLIT_SEQS;
-    o->ctas = SPLIT_CTAS;
+    o->ctas = split_ctas(c.head_dim, o->nt);
     o->part_bytes = o->split ? (int64_t) o->ctas * 2 * 8 * o->nt * (c.head_dim + 2) * 4 : 0;
     o->grid = (unsigned)(o->split ? o->ctas : items);
     return true;
 }
+// The shared memory limit of a kernel, raised once per device.
+template <auto F> cudaError_t allow_smem(int bytes, int device) {
+    static std::atomic<uint64_t> done{0};   // one for each kernel F
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(F, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 template <class T, bool E4M3, int D, int NT>
 cudaError_t attend_launch(const K8AttendArgs & a, const K8Plan & p, cudaStream_t st) {
-    constexpr int NW = 4, join = k8_join_bytes<D, NT, NW>();
+    constexpr int base = k8_smem_bytes<D, NT, NW>();
     if (!p.split) {
-        auto f = k_kv8_attend_whole<T, E4M3, D, NT, NW>;
-        if (join > 48 * 1024) {
-            const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, join);
-            if (e != cudaSuccess) return e;
-        }
-        f<<<p.grid, NW * 32, join, st>>>(a);
+        constexpr auto f = k_kv8_attend_whole<T, E4M3, D, NT, NW>;
+        const cudaError_t e = allow_smem<f>(base, a.c.device);
+        if (e != cudaSuccess) return e;
+        f<<<p.grid, NW * 32, base, st>>>(a);
         return cudaGetLastError();
     }
-    auto f = k_kv8_attend_split<T, E4M3, D, NT, NW>;
-    const int smem = join + (a.c.n_seqs + 1) * 8;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, join + (K8_MAX_SPLIT_SEQS + 1) * 8);
-        if (e != cudaSuccess) return e;
-    }
+    constexpr auto f = k_kv8_attend_split<T, E4M3, D, NT, NW>;
+    const int smem = base + (a.c.n_seqs + 1) * 8;
+    cudaError_t e = allow_smem<f>(base + (K8_MAX_SPLIT_SEQS + 1) * 8, a.c.device);
+    if (e != cudaSuccess) return e;
     f<<<p.grid, NW * 32, smem, st>>>(a);
-    k_kv8_join<T, D, NT><<<(unsigned)(a.c.n_seqs * a.c.n_kv_heads), 128, 0, st>>>(a);
-    return cudaGetLastError();
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    // the join may become resident while the split kernel runs; it waits for its results
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((int64_t) a.c.n_seqs * a.c.n_kv_heads * a.max_q * (a.n_heads / a.c.n_kv_heads)));
+    cfg.blockDim = dim3(K8_JOIN_WARPS * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_kv8_join<T, D, NT>, a);
 }
 
 }  // namespace

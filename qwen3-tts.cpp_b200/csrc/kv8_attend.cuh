@@ -43,12 +43,12 @@ __device__ __forceinline__ void k8_span(const K8Seq & s, int i, int window, int 
 // is the output, O^T = V^T P^T (16 dims x 8 rows): with one query token a group of
 // G <= 8 heads fills one MMA column tile, where the usual orientation would pad it
 // to 16.  An MMA's inner index may be permuted freely if both operands agree, so a
-// lane loads what it needs straight from the page as 16-byte words:
+// lane copies what it needs straight from the page, in 16-byte words:
 //   K: lane (g, t) = (lane / 4, lane % 4) holds 16 consecutive dims of keys g and g + 8
 //      per 64 dims; word w of them is one k-step (4 dims a lane).
 //   V: the lane holds D / 8 dims (from 16 g on, per 128) of tokens 2t, 2t+1, 2t+8, 2t+9;
 //      dims 2j and 2j+1 of them are rows g and g + 8 of output tile j.
-// No shared memory or transposition is needed between the page and the MMA.
+// So nothing is exchanged or transposed between the page and the MMA.
 __device__ __forceinline__ uint32_t k8_prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
 // Four codes -> two F16 pairs (bytes 0, 1 and 2, 3).
 template <bool E4M3> __device__ __forceinline__ void k8_f16x4(uint32_t w, uint32_t & lo, uint32_t & hi);
@@ -84,42 +84,56 @@ __device__ __forceinline__ uint32_t k8_transpose(uint32_t x) {   // an 8 x 8 mat
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint4 k8_ld16(const uint8_t * p) { return ld_stream(p); }
-__device__ __forceinline__ uint2 k8_ld8b(const uint8_t * p) {
-    uint2 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-    return r;
+__device__ __forceinline__ void k8_copy16(uint32_t dst, const uint8_t * src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void k8_copy8(uint32_t dst, const uint8_t * src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void k8_copy4(uint32_t dst, const float * src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void k8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void k8_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// One block's K words of a lane: keys g and g + 8, D / 16 words each.
-template <int D> struct K8K { uint32_t a[D / 16], b[D / 16]; };
-template <int D> __device__ __forceinline__ void k8_load_k(K8K<D> & k, const uint8_t * base, int lane) {
-    const uint8_t * p = base + (lane >> 2) * D + (lane & 3) * 16;
+// A slot of a warp's ring in shared memory: one block's codes, every lane's own words
+// at its own place (word i of lane l at 16 (32 i + l): no bank conflicts, and a lane
+// waits for its own copies only), then the block's two scales.
+template <int D> struct K8Slot {
+    static constexpr int kw = D / 32;                       // 16-byte words of K a lane
+    static constexpr int vw = D == 64 ? 4 : D / 32;         // words of V a lane (8 bytes each at D = 64)
+    static constexpr int v_at = kw * 512, s_at = v_at + (D == 64 ? vw * 256 : vw * 512), bytes = s_at + 16;
+};
+template <int D> __device__ __forceinline__ void k8_fetch(uint32_t slot, const K8AttendArgs & a, int64_t page, int h, int block, int lane) {
+    const int H = a.c.n_kv_heads, g = lane >> 2, t = lane & 3;
+    const int64_t at = k8_code_off(page, h, block * K8_BLOCK, H, D);
+    const uint8_t * k = static_cast<const uint8_t *>(a.c.k) + at + g * D + t * 16;
+    const uint8_t * v = static_cast<const uint8_t *>(a.c.v) + at + 2 * t * D + (D == 64 ? g * 8 : g * 16);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
-        const uint4 x = k8_ld16(p + c * 64), y = k8_ld16(p + 8 * D + c * 64);
-        k.a[4 * c] = x.x; k.a[4 * c + 1] = x.y; k.a[4 * c + 2] = x.z; k.a[4 * c + 3] = x.w;
-        k.b[4 * c] = y.x; k.b[4 * c + 1] = y.y; k.b[4 * c + 2] = y.z; k.b[4 * c + 3] = y.w;
+        k8_copy16(slot + (2 * c) * 512 + lane * 16, k + c * 64);
+        k8_copy16(slot + (2 * c + 1) * 512 + lane * 16, k + 8 * D + c * 64);
     }
-}
-// One block's V words: tokens 2t, 2t+1, 2t+8, 2t+9, D / 32 words each.
-template <int D> struct K8V { uint32_t w[4][D / 32]; };
-template <int D> __device__ __forceinline__ void k8_load_v(K8V<D> & v, const uint8_t * base, int lane) {
-    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint8_t * p = base + (2 * t + (i & 1) + (i >> 1) * 8) * D;
-        if constexpr (D == 64) {
-            const uint2 x = k8_ld8b(p + g * 8);
-            v.w[i][0] = x.x; v.w[i][1] = x.y;
-        } else {
+        const uint8_t * p = v + ((i & 1) + (i >> 1) * 8) * D;
+        if constexpr (D == 64) k8_copy8(slot + K8Slot<D>::v_at + i * 256 + lane * 8, p);
+        else {
 #pragma unroll
-            for (int c = 0; c < D / 128; ++c) {
-                const uint4 x = k8_ld16(p + c * 128 + g * 16);
-                v.w[i][4 * c] = x.x; v.w[i][4 * c + 1] = x.y; v.w[i][4 * c + 2] = x.z; v.w[i][4 * c + 3] = x.w;
-            }
+            for (int c = 0; c < D / 128; ++c) k8_copy16(slot + K8Slot<D>::v_at + (i * (D / 128) + c) * 512 + lane * 16, p + c * 128);
         }
     }
+    if (lane < 2) k8_copy4(slot + K8Slot<D>::s_at + lane * 4, (lane ? a.c.v_scale : a.c.k_scale) + k8_scale_off(page, h, block, H));
+}
+__device__ __forceinline__ uint4 k8_lds16(uint32_t p) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(p) : "memory");
+    return r;
+}
+__device__ __forceinline__ uint2 k8_lds8(uint32_t p) {
+    uint2 r;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(p) : "memory");
+    return r;
 }
 // The first dim of output tile j of a lane (its second one follows).
 template <int D> __device__ __forceinline__ int k8_dim(int j, int lane) {
@@ -190,50 +204,61 @@ template <int D, int NT> struct K8State {
 // Segment of one warp: blocks first, first + step, .. < last of a sequence.
 struct K8Rows { int lo[2], hi[2]; };              // keys of the lane's rows 8 nt + 2t + {0, 1}
 
+// Ring slots of a warp: enough blocks in flight to cover the latency of HBM (4 KB a
+// block at D = 128; 148 SMs at 6.4 TB/s need some 45 KB each in flight).
+template <int D, int NT> constexpr int K8_SLOTS = D == 256 ? 2 : (D == 128 ? (NT == 1 ? 3 : 4) : 6);
+
 template <bool E4M3, class T, int D, int NT>
 __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (&q)[NT], const float (&fac)[NT][2], const K8Rows (&rows)[NT],
                                           const K8AttendArgs & a, const int32_t * table, int h, int first, int last, int step, int all_lo, int all_hi,
-                                          int any_hi, int lane) {
-    const int H = a.c.n_kv_heads;
-    const uint8_t * kc = static_cast<const uint8_t *>(a.c.k), * vc = static_cast<const uint8_t *>(a.c.v);
-    if (first >= last) return;
-    K8K<D> k;
-    K8V<D> v;
-    float ks = 0.0f, vs = 0.0f;
-    int page = k8_page(table, first / K8_BPP, a.c.n_pages);
-    int next = first + step < last ? k8_page(table, (first + step) / K8_BPP, a.c.n_pages) : -1;
-    auto off = [&](int pg, int X) { return k8_code_off(pg, h, X % K8_BPP * K8_BLOCK, H, D); };
-    if (page >= 0) {
-        k8_load_k<D>(k, kc + off(page, first), lane);
-        k8_load_v<D>(v, vc + off(page, first), lane);
-        ks = a.c.k_scale[k8_scale_off(page, h, first % K8_BPP, H)];
-        vs = a.c.v_scale[k8_scale_off(page, h, first % K8_BPP, H)];
-    }
-    for (int X = first; X < last; X += step) {
-        const int nX = X + step;
-        const int nnext = nX + step < last ? k8_page(table, (nX + step) / K8_BPP, a.c.n_pages) : -1;
-        const float ks0 = ks, vs0 = vs;
-        float s[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            uint32_t a0, a1, a2, a3;
-            k8_f16x4<E4M3>(k.a[i], a0, a2);
-            k8_f16x4<E4M3>(k.b[i], a1, a3);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) k8_mma(s[nt], a0, a1, a2, a3, q[nt].x[i][0], q[nt].x[i][1]);
+                                          int any_hi, uint32_t ring, int lane) {
+    constexpr int S = K8_SLOTS<D, NT>;
+    const int count = first < last ? (last - first + step - 1) / step : 0;
+    // page numbers of the next 64 blocks, two to a lane
+    auto page_of = [&](int i) { return i < count ? k8_page(table, (first + i * step) / K8_BPP, a.c.n_pages) : -1; };
+    int pg0 = page_of(lane), pg1 = page_of(lane + 32);
+    uint32_t good = 0;                              // slots that hold a block
+    auto fetch = [&](int i, int slot) {             // block i into its slot
+        good &= ~(1u << slot);
+        if (i < count) {
+            if (i && i % 32 == 0) { pg0 = pg1; pg1 = page_of(i + 32 + lane); }
+            const int page = __shfl_sync(0xffffffffu, pg0, i & 31);
+            if (page >= 0) {
+                good |= 1u << slot;
+                k8_fetch<D>(ring + slot * K8Slot<D>::bytes, a, page, h, (first + i * step) % K8_BPP, lane);
+            } else if (lane == 0) k8_flag(a.c.status, K8_BAD_PAGE);
         }
-        const bool have = page >= 0;
-        if (!have && lane == 0) k8_flag(a.c.status, K8_BAD_PAGE);
-        if (nX < last && next >= 0) {
-            k8_load_k<D>(k, kc + off(next, nX), lane);
-            ks = a.c.k_scale[k8_scale_off(next, h, nX % K8_BPP, H)];
-            vs = a.c.v_scale[k8_scale_off(next, h, nX % K8_BPP, H)];
-        }
-        if (have) {
+        k8_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S; ++i) fetch(i, i);
+    int slot = 0;
+    for (int i = 0; i < count; ++i) {
+        const int X = first + i * step;
+        const uint32_t at = ring + slot * K8Slot<D>::bytes;
+        k8_wait<S - 1>();
+        __syncwarp();                               // the scales are other lanes' copies
+        if (good >> slot & 1) {
+            const uint2 sc = k8_lds8(at + K8Slot<D>::s_at);
+            const float ks0 = __uint_as_float(sc.x), vs0 = __uint_as_float(sc.y);
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                const uint4 x = k8_lds16(at + (2 * c) * 512 + lane * 16), y = k8_lds16(at + (2 * c + 1) * 512 + lane * 16);
+                const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t a0, a1, a2, a3;
+                    k8_f16x4<E4M3>(xw[w], a0, a2);
+                    k8_f16x4<E4M3>(yw[w], a1, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) k8_mma(s[nt], a0, a1, a2, a3, q[nt].x[4 * c + w][0], q[nt].x[4 * c + w][1]);
+                }
+            }
             const bool whole = X * K8_BLOCK >= all_lo && X * K8_BLOCK + K8_BLOCK <= all_hi;   // every row sees every key
             bool up = false;
 #pragma unroll
@@ -283,36 +308,51 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
                 for (int r = 0; r < 2; ++r)   // a block that a row does not see adds nothing, even if its scale is NaN
                     fv[nt][r] = whole || (X * K8_BLOCK < rows[nt].hi[r] && X * K8_BLOCK + K8_BLOCK > rows[nt].lo[r]) ? vs0 : 0.0f;
             }
-            if (!whole) {   // rows of the page past the sequence's end may hold anything
+            // rows of the page past the sequence's end may hold anything
+            const int beyond = whole ? K8_BLOCK : any_hi - X * K8_BLOCK - 2 * (lane & 3);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (X * K8_BLOCK + 2 * (lane & 3) + (i & 1) + (i >> 1) * 8 >= any_hi)
+            for (int c = 0; c < (D + 127) / 128; ++c) {
+                uint32_t v[4][4];
+                constexpr int W = D == 64 ? 2 : 4;
 #pragma unroll
-                        for (int w = 0; w < D / 32; ++w) v.w[i][w] = 0;
-            }
-#pragma unroll
-            for (int w = 0; w < D / 32; ++w) {
-                uint32_t a0[2], a1[2], a2[2], a3[2];
-                // tokens' bytes side by side: [x0 y0 x1 y1], [x2 y2 x3 y3]
-                k8_f16x4<E4M3>(k8_prmt(v.w[0][w], v.w[1][w], 0x5140), a0[0], a1[0]);
-                k8_f16x4<E4M3>(k8_prmt(v.w[0][w], v.w[1][w], 0x7362), a0[1], a1[1]);
-                k8_f16x4<E4M3>(k8_prmt(v.w[2][w], v.w[3][w], 0x5140), a2[0], a3[0]);
-                k8_f16x4<E4M3>(k8_prmt(v.w[2][w], v.w[3][w], 0x7362), a2[1], a3[1]);
-#pragma unroll
-                for (int o = 0; o < 2; ++o)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        k8_mma(c, a0[o], a1[o], a2[o], a3[o], p[nt][0], p[nt][1]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) st.o[nt][2 * w + o][e] = fmaf(c[e], fv[nt][e & 1], st.o[nt][2 * w + o][e]);
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (D == 64) {
+                        const uint2 x = k8_lds8(at + K8Slot<D>::v_at + i * 256 + lane * 8);
+                        v[i][0] = x.x; v[i][1] = x.y;
+                    } else {
+                        const uint4 x = k8_lds16(at + K8Slot<D>::v_at + (i * (D / 128) + c) * 512 + lane * 16);
+                        v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
                     }
+                    if (!whole && (i & 1) + (i >> 1) * 8 >= beyond)
+#pragma unroll
+                        for (int w = 0; w < W; ++w) v[i][w] = 0;
+                }
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    uint32_t a0[2], a1[2], a2[2], a3[2];
+                    // tokens' bytes side by side: [x0 y0 x1 y1], [x2 y2 x3 y3]
+                    k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x5140), a0[0], a1[0]);
+                    k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x7362), a0[1], a1[1]);
+                    k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x5140), a2[0], a3[0]);
+                    k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x7362), a2[1], a3[1]);
+#pragma unroll
+                    for (int o = 0; o < 2; ++o)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            k8_mma(d, a0[o], a1[o], a2[o], a3[o], p[nt][0], p[nt][1]);
+                            const int j = c * 8 + 2 * w + o;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) st.o[nt][j][e] = fmaf(d[e], fv[nt][e & 1], st.o[nt][j][e]);
+                        }
+                }
             }
         }
-        if (nX < last && next >= 0) k8_load_v<D>(v, vc + off(next, nX), lane);
-        page = next;
-        next = nnext;
+        __syncwarp();                               // the slot has been read
+        fetch(i + S, slot);
+        slot = slot + 1 == S ? 0 : slot + 1;
     }
+    k8_wait<0>();
 }
 
 // What a CTA of the split kernel leaves of an item it has only a part of:
@@ -370,8 +410,10 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq &
             for (int j = 0; j < D / 16; ++j) st.o[nt][j][i] = st.o[nt][j][i + 2] = 0.0f;
         }
     const int X0 = max(pg0 * K8_BPP, lo / K8_BLOCK), X1 = min(pg1 * K8_BPP, (hi1 + K8_BLOCK - 1) / K8_BLOCK);
-    k8_blocks<E4M3, T, D, NT>(st, q, fac, rows, a, a.table + (int64_t) b * a.c.max_pages, h, X0 + warp, X1, NW, lo1, hi, hi1, lane);
-    // join: rows' sums over lanes, then the warps through shared memory
+    k8_blocks<E4M3, T, D, NT>(st, q, fac, rows, a, a.table + (int64_t) b * a.c.max_pages, h, X0 + warp, X1, NW, lo1, hi, hi1,
+                              smem_u32(smem) + warp * K8_SLOTS<D, NT> * K8Slot<D>::bytes, lane);
+    // join: rows' sums over lanes, then the warps through the shared memory that held the rings
+    __syncthreads();
     float * sm = smem, * sl = smem + NW * 8 * NT, * so = smem + 2 * NW * 8 * NT;   // [NW][8 NT] twice, [NW][8 NT][D + 4]
     constexpr int LD = D + 4;
 #pragma unroll
@@ -412,11 +454,14 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq &
     }
     __syncthreads();
 }
-template <int D, int NT, int NW> __host__ __device__ constexpr int k8_join_bytes() { return (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4; }
+template <int D, int NT, int NW> __host__ __device__ constexpr int k8_smem_bytes() {
+    return (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4 > NW * K8_SLOTS<D, NT> * K8Slot<D>::bytes ? (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4
+                                                                                               : NW * K8_SLOTS<D, NT> * K8Slot<D>::bytes;
+}
 
 // One CTA per (sequence, kv head, row tile).
 template <class T, bool E4M3, int D, int NT, int NW>
-__global__ void __launch_bounds__(NW * 32) k_kv8_attend_whole(K8AttendArgs a) {
+__global__ void __launch_bounds__(NW * 32, D == 256 ? 2 : (NT == 1 ? 4 : (NT == 2 ? 3 : 2))) k_kv8_attend_whole(K8AttendArgs a) {
     extern __shared__ __align__(16) float k8_smem[];
     const int H = a.c.n_kv_heads, G = a.n_heads / H;
     const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles % H, b = blockIdx.x / a.tiles / H;
@@ -468,10 +513,11 @@ __device__ __forceinline__ long long k8_chunk(long long total, int ctas) {
 }
 
 template <class T, bool E4M3, int D, int NT, int NW>
-__global__ void __launch_bounds__(NW * 32) k_kv8_attend_split(K8AttendArgs a) {
+__global__ void __launch_bounds__(NW * 32, D == 256 ? 2 : (NT == 1 ? 4 : (NT == 2 ? 3 : 2))) k_kv8_attend_split(K8AttendArgs a) {
     extern __shared__ __align__(16) float k8_smem[];
     __shared__ long long s_carry[NW];
-    long long * at = reinterpret_cast<long long *>(k8_smem + k8_join_bytes<D, NT, NW>() / 4);
+    pdl_trigger();
+    long long * at = reinterpret_cast<long long *>(k8_smem + k8_smem_bytes<D, NT, NW>() / 4);
     k8_line<NT, NW * 32>(a, at, s_carry);
     const long long total = at[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
     long long pos = blockIdx.x * chunk;
@@ -496,39 +542,61 @@ __global__ void __launch_bounds__(NW * 32) k_kv8_attend_split(K8AttendArgs a) {
     }
 }
 
-// Joins the parts of an item in the order of the cache, one CTA per (sequence, kv head);
-// rows of items without pages become zeros.
+// Joins the parts of an item: one CTA per (sequence, kv head, row of the tile), its
+// warps take the parts in turn (a lane holds D / 32 dims) and are joined in warp
+// order, so the order of the sums is fixed.  Rows of items without pages become zeros.
+constexpr int K8_JOIN_WARPS = 8;
 template <class T, int D, int NT>
-__global__ void __launch_bounds__(128) k_kv8_join(K8AttendArgs a) {
-    __shared__ long long at[K8_MAX_SPLIT_SEQS + 1], s_carry[4];
-    const int H = a.c.n_kv_heads, G = a.n_heads / H, h = blockIdx.x % H, b = blockIdx.x / H;
-    k8_line<NT, 128>(a, at, s_carry);
+__global__ void __launch_bounds__(K8_JOIN_WARPS * 32) k_kv8_join(K8AttendArgs a) {
+    __shared__ long long at[K8_MAX_SPLIT_SEQS + 1], s_carry[K8_JOIN_WARPS];
+    __shared__ float s_m[K8_JOIN_WARPS], s_l[K8_JOIN_WARPS], s_o[K8_JOIN_WARPS][D];
+    constexpr int V = D / 32;
+    const int H = a.c.n_kv_heads, G = a.n_heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rr = blockIdx.x % (a.max_q * G), h = blockIdx.x / (a.max_q * G) % H, b = blockIdx.x / (a.max_q * G) / H;
+    k8_line<NT, K8_JOIN_WARPS * 32>(a, at, s_carry);
+    pdl_wait();                                     // every CTA, so that the join does not end before the split kernel
     const long long total = at[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
     const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
+    if (rr >= s.n * G) return;
     int pg0, pg1;
     k8_pages(s, a.window, pg0, pg1);
-    const int np = pg1 - pg0, tiles = (s.n * G + 8 * NT - 1) / (8 * NT);
-    for (int tile = 0; tile < tiles; ++tile) {
-        const long long p0 = at[b] + (long long)(h * tiles + tile) * np, p1 = p0 + np;
-        const int c0 = (int)(p0 / chunk), c1 = np ? (int)((p1 - 1) / chunk) : c0 - 1;
-        if (c0 == c1) continue;
-        for (int e = threadIdx.x; e < 8 * NT * D; e += 128) {
-            const int r = e / D, d = e % D, rr = tile * 8 * NT + r;
-            if (rr >= s.n * G) break;
-            float m = -INFINITY, l = 0.0f, o = 0.0f;
-            auto slot = [&](int c) { return a.part + ((long long) c * 2 + (c == c0 && p0 > c * chunk ? 1 : 0)) * K8Part<D, NT>::floats; };
-            for (int c = c0; c <= c1; ++c) m = fmaxf(m, slot(c)[r]);
-            for (int c = c0; c <= c1; ++c) {
-                const float * p = slot(c);
-                const float f = p[r] == m ? 1.0f : k8_exp2(p[r] - m);
-                l = fmaf(p[8 * NT + r], f, l);
-                o = fmaf(p[16 * NT + r * D + d], f, o);
-            }
-            const int row = s.row0 + rr / G, hq = h * G + rr % G;
-            k8_write_row<T>(a, row, hq, d, o, l == 0.0f ? 0.0f : 1.0f / l);
-            if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = l == 0.0f ? -INFINITY : (m - K8_LIFT + log2f(l)) * 0.693147180559945309417f;
-        }
+    const int np = pg1 - pg0, tiles = (s.n * G + 8 * NT - 1) / (8 * NT), tile = rr / (8 * NT), r = rr % (8 * NT);
+    const long long p0 = at[b] + (long long)(h * tiles + tile) * np, p1 = p0 + np;
+    const int c0 = (int)(p0 / chunk), c1 = np ? (int)((p1 - 1) / chunk) : c0 - 1;
+    if (c0 == c1) return;                           // one CTA had all of it
+    float m = -INFINITY, l = 0.0f, o[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = 0.0f;
+#pragma unroll 4
+    for (int c = c0 + warp; c <= c1; c += K8_JOIN_WARPS) {
+        const float * p = a.part + ((long long) c * 2 + (c == c0 && p0 > c * chunk ? 1 : 0)) * K8Part<D, NT>::floats;
+        struct alignas(V * 4 > 16 ? 16 : V * 4) Vec { float x[V]; };
+        const Vec x = *reinterpret_cast<const Vec *>(p + 16 * NT + r * D + lane * V);
+        const float mc = p[r], lc = p[8 * NT + r], mn = fmaxf(m, mc);
+        const float f = m == mn ? 1.0f : k8_exp2(m - mn), fc = mc == mn ? 1.0f : k8_exp2(mc - mn);
+        m = mn;
+        l = l * f + lc * fc;
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = o[e] * f + x.x[e] * fc;
     }
+    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+#pragma unroll
+    for (int e = 0; e < V; ++e) s_o[warp][lane * V + e] = o[e];
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    const int d = threadIdx.x;
+    float M = -INFINITY, L = 0.0f, O = 0.0f;
+#pragma unroll
+    for (int w = 0; w < K8_JOIN_WARPS; ++w) M = fmaxf(M, s_m[w]);
+#pragma unroll
+    for (int w = 0; w < K8_JOIN_WARPS; ++w) {
+        const float f = s_m[w] == M ? 1.0f : k8_exp2(s_m[w] - M);
+        L = fmaf(s_l[w], f, L);
+        O = fmaf(s_o[w][d], f, O);
+    }
+    const int row = s.row0 + rr / G, hq = h * G + rr % G;
+    k8_write_row<T>(a, row, hq, d, O, L == 0.0f ? 0.0f : 1.0f / L);
+    if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = L == 0.0f ? -INFINITY : (M - K8_LIFT + log2f(L)) * 0.693147180559945309417f;
 }
 
 // Accumulated weights, plain: one warp per (sequence, kv head, key), rows and heads in order.
