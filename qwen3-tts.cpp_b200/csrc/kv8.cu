@@ -121,11 +121,6 @@ template <class F> void by_cache(const qtts_kv8 & c, F f) {
 // ranges are split evenly over the GPU.
 struct K8Plan { int nt, tiles, split, ctas; int64_t part_bytes; unsigned grid; };
 constexpr int SMS = 148, NW = 4;
-// CTAs of the split kernel that are resident together (registers, then shared memory)
-int split_ctas(int dim, int nt) {
-    const int per = dim == 256 ? 2 : (nt == 1 ? 4 : (nt == 2 ? 3 : 2));
-    return SMS * per;
-}
 bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     const int64_t R = (int64_t) p.max_q * (p.n_heads / c.n_kv_heads);
     o->nt = R <= 8 ? 1 : (R <= 16 || c.head_dim == 256 ? 2 : 4);
@@ -133,7 +128,7 @@ bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     if (items > 0x7fffffff) return false;
     o->tiles = (int) tiles;
     o->split = c.max_pages > 8 && R <= 64 && c.n_seqs <= K8_MAX_SPLIT_SEQS;
-    o->ctas = split_ctas(c.head_dim, o->nt);
+    o->ctas = SMS * k8_ctas_per_sm(c.head_dim, o->nt);
     o->part_bytes = o->split ? (int64_t) o->ctas * 2 * 8 * o->nt * (c.head_dim + 2) * 4 : 0;
     o->grid = (unsigned)(o->split ? o->ctas : items);
     return true;

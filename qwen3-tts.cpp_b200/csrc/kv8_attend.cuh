@@ -96,34 +96,37 @@ __device__ __forceinline__ void k8_copy4(uint32_t dst, const float * src) {
 __device__ __forceinline__ void k8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void k8_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// A slot of a warp's ring in shared memory: one block's codes, every lane's own words
-// at its own place (word i of lane l at 16 (32 i + l): no bank conflicts, and a lane
-// waits for its own copies only), then the block's two scales.
-template <int D> struct K8Slot {
-    static constexpr int kw = D / 32;                       // 16-byte words of K a lane
-    static constexpr int vw = D == 64 ? 4 : D / 32;         // words of V a lane (8 bytes each at D = 64)
-    static constexpr int v_at = kw * 512, s_at = v_at + (D == 64 ? vw * 256 : vw * 512), bytes = s_at + 16;
+// A slot of a warp's ring in shared memory: the codes of U blocks, every lane's own
+// words at its own place (word i of lane l at 16 (32 i + l): no bank conflicts, and a
+// lane waits for its own copies only), then the blocks' scales.
+template <int D, int U> struct K8Slot {
+    static constexpr int k_bytes = D * 16, v_bytes = D * 16, block = k_bytes + v_bytes, s_at = U * block, bytes = s_at + 16;
 };
-template <int D> __device__ __forceinline__ void k8_fetch(uint32_t slot, const K8AttendArgs & a, int64_t page, int h, int block, int lane) {
+template <int D, int U> __device__ __forceinline__ void k8_fetch(uint32_t slot, const K8AttendArgs & a, int page, int h, int block, int lane) {
     const int H = a.c.n_kv_heads, g = lane >> 2, t = lane & 3;
     const int64_t at = k8_code_off(page, h, block * K8_BLOCK, H, D);
     const uint8_t * k = static_cast<const uint8_t *>(a.c.k) + at + g * D + t * 16;
     const uint8_t * v = static_cast<const uint8_t *>(a.c.v) + at + 2 * t * D + (D == 64 ? g * 8 : g * 16);
+    const uint32_t ks = slot + lane * 16, vs = slot + K8Slot<D, U>::k_bytes + lane * (D == 64 ? 8 : 16);
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-        k8_copy16(slot + (2 * c) * 512 + lane * 16, k + c * 64);
-        k8_copy16(slot + (2 * c + 1) * 512 + lane * 16, k + 8 * D + c * 64);
-    }
+    for (int u = 0; u < U; ++u) {
+        constexpr int B = K8Slot<D, U>::block;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint8_t * p = v + ((i & 1) + (i >> 1) * 8) * D;
-        if constexpr (D == 64) k8_copy8(slot + K8Slot<D>::v_at + i * 256 + lane * 8, p);
-        else {
+        for (int c = 0; c < D / 64; ++c) {
+            k8_copy16(ks + u * B + (2 * c) * 512, k + u * K8_BLOCK * D + c * 64);
+            k8_copy16(ks + u * B + (2 * c + 1) * 512, k + u * K8_BLOCK * D + 8 * D + c * 64);
+        }
 #pragma unroll
-            for (int c = 0; c < D / 128; ++c) k8_copy16(slot + K8Slot<D>::v_at + (i * (D / 128) + c) * 512 + lane * 16, p + c * 128);
+        for (int i = 0; i < 4; ++i) {
+            const uint8_t * p = v + (u * K8_BLOCK + (i & 1) + (i >> 1) * 8) * D;
+            if constexpr (D == 64) k8_copy8(vs + u * B + i * 256, p);
+            else {
+#pragma unroll
+                for (int c = 0; c < D / 128; ++c) k8_copy16(vs + u * B + (i * (D / 128) + c) * 512, p + c * 128);
+            }
         }
     }
-    if (lane < 2) k8_copy4(slot + K8Slot<D>::s_at + lane * 4, (lane ? a.c.v_scale : a.c.k_scale) + k8_scale_off(page, h, block, H));
+    if (lane < 2 * U) k8_copy4(slot + K8Slot<D, U>::s_at + lane * 4, (lane & 1 ? a.c.v_scale : a.c.k_scale) + k8_scale_off(page, h, block + (lane >> 1), H));
 }
 __device__ __forceinline__ uint4 k8_lds16(uint32_t p) {
     uint4 r;
@@ -189,43 +192,47 @@ __device__ __forceinline__ float k8_load_q(K8Q<T, D> & q, const T * row, int lan
 }
 
 // ---- few rows ----------------------------------------------------------------
-// One warp's running state over its blocks: reference value m (log2 units) and sum
-// per row, unnormalised output.  The reference moves only when a score passes it by
-// more than 4 (a vote), so most blocks need no reduction over lanes; weights are
-// 2^(s - m + 8), at most 2^12 and in F16's normal range down to 2^-22 of the
-// largest.  They are rounded to F16 for the product with V (half a step is 2^-12
-// relative, independent from key to key, under the output's own rounding); their
-// sum is taken before that, in F32.
-constexpr float K8_LIFT = 8.0f, K8_SLACK = 4.0f;
+// One warp's running state over its blocks: per row a reference value m (log2 units)
+// and the sum of the weights 2^(s - m + 8), and the output in units of `unit`, a V
+// scale.  References move only when a score passes m by more than 4, or a block's V
+// scale passes `unit` more than 8 times: most blocks need a vote and no reduction over
+// lanes.  A weight times its block's V scale over `unit`, at most 2^15, is rounded to
+// F16 for the product with V: half a step is 2^-12 relative, independent from key to
+// key and under the output's own rounding, or 2^-33 of the largest weight times the
+// largest V scale.  The sum of the weights is taken before that, in F32.
+constexpr float K8_LIFT = 8.0f, K8_SLACK = 4.0f, K8_UNIT_SLACK = 8.0f, K8_UNIT_MIN = 7.8886090522101181e-31f;   // 2^-100
 template <int D, int NT> struct K8State {
     float m[NT][2], l[NT][2], o[NT][D / 16][4];   // rows 8 nt + 2t, + 1
+    float unit;
 };
-
-// Segment of one warp: blocks first, first + step, .. < last of a sequence.
 struct K8Rows { int lo[2], hi[2]; };              // keys of the lane's rows 8 nt + 2t + {0, 1}
 
-// Ring slots of a warp: enough blocks in flight to cover the latency of HBM (4 KB a
-// block at D = 128; 148 SMs at 6.4 TB/s need some 45 KB each in flight).
-template <int D, int NT> constexpr int K8_SLOTS = D == 256 ? 2 : (D == 128 ? (NT == 1 ? 3 : 4) : 6);
+// Blocks that a warp works on together (independent chains of MMAs), and its ring's
+// slots: enough bytes in flight to cover the latency of HBM (148 SMs at 6.4 TB/s need
+// some 45 KB each).
+template <int D, int NT> constexpr int K8_U = D * NT <= 128 ? 2 : 1;
+template <int D, int NT> constexpr int K8_SLOTS = D == 64 ? (NT == 1 ? 3 : 6) : (D == 128 ? (NT == 1 ? 2 : 4) : 2);
 
+// Steps first, first + step, .. < last of U blocks each.
 template <bool E4M3, class T, int D, int NT>
 __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (&q)[NT], const float (&fac)[NT][2], const K8Rows (&rows)[NT],
                                           const K8AttendArgs & a, const int32_t * table, int h, int first, int last, int step, int all_lo, int all_hi,
                                           int any_hi, uint32_t ring, int lane) {
-    constexpr int S = K8_SLOTS<D, NT>;
+    constexpr int S = K8_SLOTS<D, NT>, U = K8_U<D, NT>, KEYS = U * K8_BLOCK, SPP = K8_PAGE / KEYS;
+    using Slot = K8Slot<D, U>;
     const int count = first < last ? (last - first + step - 1) / step : 0;
-    // page numbers of the next 64 blocks, two to a lane
-    auto page_of = [&](int i) { return i < count ? k8_page(table, (first + i * step) / K8_BPP, a.c.n_pages) : -1; };
+    // page numbers of the next 64 steps, two to a lane
+    auto page_of = [&](int i) { return i < count ? k8_page(table, (first + i * step) / SPP, a.c.n_pages) : -1; };
     int pg0 = page_of(lane), pg1 = page_of(lane + 32);
-    uint32_t good = 0;                              // slots that hold a block
-    auto fetch = [&](int i, int slot) {             // block i into its slot
+    uint32_t good = 0;                              // slots that hold a step
+    auto fetch = [&](int i, int slot) {             // step i into its slot
         good &= ~(1u << slot);
         if (i < count) {
             if (i && i % 32 == 0) { pg0 = pg1; pg1 = page_of(i + 32 + lane); }
             const int page = __shfl_sync(0xffffffffu, pg0, i & 31);
             if (page >= 0) {
                 good |= 1u << slot;
-                k8_fetch<D>(ring + slot * K8Slot<D>::bytes, a, page, h, (first + i * step) % K8_BPP, lane);
+                k8_fetch<D, U>(ring + slot * Slot::bytes, a, page, h, (first + i * step) % SPP * U, lane);
             } else if (lane == 0) k8_flag(a.c.status, K8_BAD_PAGE);
         }
         k8_commit();
@@ -234,51 +241,62 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
     for (int i = 0; i < S; ++i) fetch(i, i);
     int slot = 0;
     for (int i = 0; i < count; ++i) {
-        const int X = first + i * step;
-        const uint32_t at = ring + slot * K8Slot<D>::bytes;
+        const int j0 = (first + i * step) * KEYS;   // the step's first key
+        const uint32_t at = ring + slot * Slot::bytes;
         k8_wait<S - 1>();
         __syncwarp();                               // the scales are other lanes' copies
         if (good >> slot & 1) {
-            const uint2 sc = k8_lds8(at + K8Slot<D>::s_at);
-            const float ks0 = __uint_as_float(sc.x), vs0 = __uint_as_float(sc.y);
-            float s[NT][4];
+            float ks[U], vs[U], s[U][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int u = 0; u < U; ++u) {
+                const uint2 sc = k8_lds8(at + Slot::s_at + u * 8);
+                ks[u] = __uint_as_float(sc.x);
+                vs[u] = __uint_as_float(sc.y);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-                const uint4 x = k8_lds16(at + (2 * c) * 512 + lane * 16), y = k8_lds16(at + (2 * c + 1) * 512 + lane * 16);
-                const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    uint32_t a0, a1, a2, a3;
-                    k8_f16x4<E4M3>(xw[w], a0, a2);
-                    k8_f16x4<E4M3>(yw[w], a1, a3);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) k8_mma(s[nt], a0, a1, a2, a3, q[nt].x[4 * c + w][0], q[nt].x[4 * c + w][1]);
-                }
+                    for (int e = 0; e < 4; ++e) s[u][nt][e] = 0.0f;
             }
-            const bool whole = X * K8_BLOCK >= all_lo && X * K8_BLOCK + K8_BLOCK <= all_hi;   // every row sees every key
-            bool up = false;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int c = 0; c < D / 64; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[nt][e] *= fac[nt][e & 1] * ks0;
-                    if (!whole) {
-                        const int j = X * K8_BLOCK + (lane >> 2) + (e >> 1) * 8;
-                        if (j < rows[nt].lo[e & 1] || j >= rows[nt].hi[e & 1]) s[nt][e] = -INFINITY;
+                for (int u = 0; u < U; ++u) {
+                    const uint32_t kp = at + u * Slot::block + lane * 16;
+                    const uint4 x = k8_lds16(kp + (2 * c) * 512), y = k8_lds16(kp + (2 * c + 1) * 512);
+                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t a0, a1, a2, a3;
+                        k8_f16x4<E4M3>(xw[w], a0, a2);
+                        k8_f16x4<E4M3>(yw[w], a1, a3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) k8_mma(s[u][nt], a0, a1, a2, a3, q[nt].x[4 * c + w][0], q[nt].x[4 * c + w][1]);
                     }
                 }
-                up |= fmaxf(s[nt][0], s[nt][2]) > st.m[nt][0] + K8_SLACK || fmaxf(s[nt][1], s[nt][3]) > st.m[nt][1] + K8_SLACK;
-            }
+            const bool whole = j0 >= all_lo && j0 + KEYS <= all_hi;   // every row sees every key
+            bool up = false;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[u][nt][e] *= fac[nt][e & 1] * ks[u];
+                        if (!whole) {
+                            const int j = j0 + u * K8_BLOCK + (lane >> 2) + (e >> 1) * 8;
+                            if (j < rows[nt].lo[e & 1] || j >= rows[nt].hi[e & 1]) s[u][nt][e] = -INFINITY;
+                        }
+                    }
+                    up |= fmaxf(s[u][nt][0], s[u][nt][2]) > st.m[nt][0] + K8_SLACK || fmaxf(s[u][nt][1], s[u][nt][3]) > st.m[nt][1] + K8_SLACK;
+                }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        float m = fmaxf(s[nt][r], s[nt][r + 2]);
+                        float m = fmaxf(s[0][nt][r], s[0][nt][r + 2]);
+#pragma unroll
+                        for (int u = 1; u < U; ++u) m = fmaxf(m, fmaxf(s[u][nt][r], s[u][nt][r + 2]));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -290,61 +308,75 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
                         for (int j = 0; j < D / 16; ++j) { st.o[nt][j][r] *= f; st.o[nt][j][r + 2] *= f; }
                     }
             }
-            uint32_t p[NT][2];
-            float fv[NT][2];
+            float top = vs[0];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float e[4];
+            for (int u = 1; u < U; ++u) top = fmaxf(top, vs[u]);
+            if (top > st.unit * K8_UNIT_SLACK) {    // the same for the whole warp
+                const float f = st.unit / top;
+                st.unit = top;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    e[i] = k8_exp2(s[nt][i] - st.m[nt][i & 1] + K8_LIFT);
-                    if (!whole && s[nt][i] == -INFINITY) e[i] = 0.0f;   // (-inf) - (-inf) of a row that has seen nothing yet
-                }
-                st.l[nt][0] += e[0] + e[2];
-                st.l[nt][1] += e[1] + e[3];
-                p[nt][0] = k8_transpose(k8_pack(e[0], e[1]));
-                p[nt][1] = k8_transpose(k8_pack(e[2], e[3]));
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int r = 0; r < 2; ++r)   // a block that a row does not see adds nothing, even if its scale is NaN
-                    fv[nt][r] = whole || (X * K8_BLOCK < rows[nt].hi[r] && X * K8_BLOCK + K8_BLOCK > rows[nt].lo[r]) ? vs0 : 0.0f;
+                    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) st.o[nt][j][e] *= f;
             }
-            // rows of the page past the sequence's end may hold anything
-            const int beyond = whole ? K8_BLOCK : any_hi - X * K8_BLOCK - 2 * (lane & 3);
+            const float inv = __fdividef(1.0f, st.unit);
+            uint32_t p[U][NT][2];
 #pragma unroll
-            for (int c = 0; c < (D + 127) / 128; ++c) {
-                uint32_t v[4][4];
-                constexpr int W = D == 64 ? 2 : 4;
+            for (int u = 0; u < U; ++u) {
+                const float rv = vs[u] * inv;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (D == 64) {
-                        const uint2 x = k8_lds8(at + K8Slot<D>::v_at + i * 256 + lane * 8);
-                        v[i][0] = x.x; v[i][1] = x.y;
-                    } else {
-                        const uint4 x = k8_lds16(at + K8Slot<D>::v_at + (i * (D / 128) + c) * 512 + lane * 16);
-                        v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
+                for (int nt = 0; nt < NT; ++nt) {
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = k8_exp2(s[u][nt][i] - (st.m[nt][i & 1] - K8_LIFT));
+                        // a key that a row does not see adds nothing, even before the row has seen any or if a scale is NaN
+                        const bool hidden = !whole && s[u][nt][i] == -INFINITY;
+                        st.l[nt][i & 1] += hidden ? 0.0f : x;
+                        e[i] = hidden ? 0.0f : x * rv;
                     }
-                    if (!whole && (i & 1) + (i >> 1) * 8 >= beyond)
-#pragma unroll
-                        for (int w = 0; w < W; ++w) v[i][w] = 0;
+                    p[u][nt][0] = k8_transpose(k8_pack(e[0], e[1]));
+                    p[u][nt][1] = k8_transpose(k8_pack(e[2], e[3]));
                 }
+            }
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    uint32_t a0[2], a1[2], a2[2], a3[2];
-                    // tokens' bytes side by side: [x0 y0 x1 y1], [x2 y2 x3 y3]
-                    k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x5140), a0[0], a1[0]);
-                    k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x7362), a0[1], a1[1]);
-                    k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x5140), a2[0], a3[0]);
-                    k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x7362), a2[1], a3[1]);
+            for (int u = 0; u < U; ++u) {
+                // rows of the page past the sequence's end may hold anything
+                const int beyond = whole ? K8_BLOCK : any_hi - j0 - u * K8_BLOCK - 2 * (lane & 3);
+                const uint32_t vp = at + u * Slot::block + Slot::k_bytes + lane * (D == 64 ? 8 : 16);
 #pragma unroll
-                    for (int o = 0; o < 2; ++o)
+                for (int c = 0; c < (D + 127) / 128; ++c) {
+                    uint32_t v[4][4];
+                    constexpr int W = D == 64 ? 2 : 4;
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            k8_mma(d, a0[o], a1[o], a2[o], a3[o], p[nt][0], p[nt][1]);
-                            const int j = c * 8 + 2 * w + o;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) st.o[nt][j][e] = fmaf(d[e], fv[nt][e & 1], st.o[nt][j][e]);
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (D == 64) {
+                            const uint2 x = k8_lds8(vp + i * 256);
+                            v[i][0] = x.x; v[i][1] = x.y;
+                        } else {
+                            const uint4 x = k8_lds16(vp + (i * (D / 128) + c) * 512);
+                            v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
                         }
+                        if (!whole && (i & 1) + (i >> 1) * 8 >= beyond)
+#pragma unroll
+                            for (int w = 0; w < W; ++w) v[i][w] = 0;
+                    }
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        uint32_t a0[2], a1[2], a2[2], a3[2];
+                        // tokens' bytes side by side: [x0 y0 x1 y1], [x2 y2 x3 y3]
+                        k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x5140), a0[0], a1[0]);
+                        k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x7362), a0[1], a1[1]);
+                        k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x5140), a2[0], a3[0]);
+                        k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x7362), a2[1], a3[1]);
+#pragma unroll
+                        for (int o = 0; o < 2; ++o)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                k8_mma(st.o[nt][c * 8 + 2 * w + o], a0[o], a1[o], a2[o], a3[o], p[u][nt][0], p[u][nt][1]);
+                    }
                 }
             }
         }
@@ -373,7 +405,7 @@ template <class T> __device__ __forceinline__ void k8_write_row(const K8AttendAr
 }
 
 // One segment (pages of one (sequence, kv head, row tile)) by the whole CTA: the
-// warps take its 16-key blocks in turn, their states are joined in shared memory in
+// warps take its blocks in turn, their states are joined in shared memory in
 // warp order.  `dst` null: the item is complete and goes to out and lse.
 template <class T, bool E4M3, int D, int NT, int NW>
 __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq & s, int b, int h, int tile, int pg0, int pg1, float * dst, float * smem) {
@@ -400,6 +432,7 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq &
     k8_span(s, r0 / G, a.window, lo, hi);
     k8_span(s, min(r0 + 8 * NT - 1, R - 1) / G, a.window, lo1, hi1);
     K8State<D, NT> st;
+    st.unit = K8_UNIT_MIN;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -409,9 +442,10 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq &
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) st.o[nt][j][i] = st.o[nt][j][i + 2] = 0.0f;
         }
-    const int X0 = max(pg0 * K8_BPP, lo / K8_BLOCK), X1 = min(pg1 * K8_BPP, (hi1 + K8_BLOCK - 1) / K8_BLOCK);
+    constexpr int KEYS = K8_U<D, NT> * K8_BLOCK;
+    const int X0 = max(pg0 * (K8_PAGE / KEYS), lo / KEYS), X1 = min(pg1 * (K8_PAGE / KEYS), (hi1 + KEYS - 1) / KEYS);
     k8_blocks<E4M3, T, D, NT>(st, q, fac, rows, a, a.table + (int64_t) b * a.c.max_pages, h, X0 + warp, X1, NW, lo1, hi, hi1,
-                              smem_u32(smem) + warp * K8_SLOTS<D, NT> * K8Slot<D>::bytes, lane);
+                              smem_u32(smem) + warp * K8_SLOTS<D, NT> * K8Slot<D, K8_U<D, NT>>::bytes, lane);
     // join: rows' sums over lanes, then the warps through the shared memory that held the rings
     __syncthreads();
     float * sm = smem, * sl = smem + NW * 8 * NT, * so = smem + 2 * NW * 8 * NT;   // [NW][8 NT] twice, [NW][8 NT][D + 4]
@@ -428,7 +462,7 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq &
             if (lane < 4) { sm[warp * 8 * NT + r] = st.m[nt][i]; sl[warp * 8 * NT + r] = l; }
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
-                *reinterpret_cast<float2 *>(so + (warp * 8 * NT + r) * LD + k8_dim<D>(j, lane)) = make_float2(st.o[nt][j][i], st.o[nt][j][i + 2]);
+                *reinterpret_cast<float2 *>(so + (warp * 8 * NT + r) * LD + k8_dim<D>(j, lane)) = make_float2(st.o[nt][j][i] * st.unit, st.o[nt][j][i + 2] * st.unit);
         }
     __syncthreads();
     for (int e = threadIdx.x; e < 8 * NT * D; e += NW * 32) {
@@ -455,13 +489,16 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq &
     __syncthreads();
 }
 template <int D, int NT, int NW> __host__ __device__ constexpr int k8_smem_bytes() {
-    return (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4 > NW * K8_SLOTS<D, NT> * K8Slot<D>::bytes ? (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4
-                                                                                               : NW * K8_SLOTS<D, NT> * K8Slot<D>::bytes;
+    return (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4 > NW * K8_SLOTS<D, NT> * K8Slot<D, K8_U<D, NT>>::bytes ? (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4
+                                                                                               : NW * K8_SLOTS<D, NT> * K8Slot<D, K8_U<D, NT>>::bytes;
 }
+
+// CTAs of 4 warps that are resident together, by their registers.
+__host__ __device__ constexpr int k8_ctas_per_sm(int dim, int nt) { return dim * nt <= 64 ? 4 : (dim * nt <= 128 ? 3 : 2); }
 
 // One CTA per (sequence, kv head, row tile).
 template <class T, bool E4M3, int D, int NT, int NW>
-__global__ void __launch_bounds__(NW * 32, D == 256 ? 2 : (NT == 1 ? 4 : (NT == 2 ? 3 : 2))) k_kv8_attend_whole(K8AttendArgs a) {
+__global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_whole(K8AttendArgs a) {
     extern __shared__ __align__(16) float k8_smem[];
     const int H = a.c.n_kv_heads, G = a.n_heads / H;
     const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles % H, b = blockIdx.x / a.tiles / H;
@@ -513,7 +550,7 @@ __device__ __forceinline__ long long k8_chunk(long long total, int ctas) {
 }
 
 template <class T, bool E4M3, int D, int NT, int NW>
-__global__ void __launch_bounds__(NW * 32, D == 256 ? 2 : (NT == 1 ? 4 : (NT == 2 ? 3 : 2))) k_kv8_attend_split(K8AttendArgs a) {
+__global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_split(K8AttendArgs a) {
     extern __shared__ __align__(16) float k8_smem[];
     __shared__ long long s_carry[NW];
     pdl_trigger();
