@@ -317,7 +317,7 @@ int32_t qtts_rope_freqs(int32_t scaling, int32_t rot, double theta, double facto
  * is not finite reads back as NaN.  Kernels check every page number, length and
  * row range of the device arrays against these sizes: what does not fit is left
  * out and sets a bit of *status (1 page, 2 length, 4 rows, 8 a page of dst_table
- * that is in use), which the caller may read and clear when it likes. */
+ * that is in use, 16 a copy that did not arrive in time), which the caller may read and clear when it likes. */
 typedef struct qtts_kv8 {
     int32_t device;
     int32_t code;                     /* 0 int8, 1 e4m3 */

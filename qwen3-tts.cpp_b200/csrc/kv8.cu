@@ -51,6 +51,7 @@ const char * bad_cache(const qtts_kv8 * c) {
     if (c->n_kv_heads < 1 || c->n_kv_heads > 1024) return "n_kv_heads";
     if (c->n_pages < 1 || c->n_seqs < 0 || c->n_seqs > 65535) return "n_pages or n_seqs";
     if (c->max_pages < 1 || c->max_pages > (1 << 24)) return "max_pages";   // positions below 2^30
+    if ((int64_t) c->n_pages * c->n_kv_heads * K8_PAGE > 0x7fffffff) return "the pool has 2^31 rows at most";
     if (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->k_open || !c->v_open) return "a buffer of the cache is NULL";
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16) ||
         !aligned(c->k_open, 16) || !aligned(c->v_open, 16))
@@ -142,21 +143,42 @@ template <auto F> cudaError_t allow_smem(int bytes, int device) {
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return e;
 }
+// A pool as TMA sees it: rows of D bytes, boxes of `rows` x min(D, 128) bytes, swizzled
+// over a row's length.
+bool make_map(CUtensorMap * map, void * pool, const qtts_kv8 & c, int rows) {
+    static const auto encode = [] {
+        void * f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(f);
+    }();
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t) c.head_dim, (cuuint64_t) c.n_pages * c.n_kv_heads * K8_PAGE}, strides[1] = {(cuuint64_t) c.head_dim};
+    const cuuint32_t box[2] = {(cuuint32_t)(c.head_dim < 128 ? c.head_dim : 128), (cuuint32_t) rows}, one[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  c.head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 template <class T, bool E4M3, int D, int NT>
 cudaError_t attend_launch(const K8AttendArgs & a, const K8Plan & p, cudaStream_t st) {
+    K8Maps maps;
+    constexpr int rows = K8_U<D, NT> * K8_BLOCK;
+    if (!make_map(&maps.k, a.c.k, a.c, rows) || !make_map(&maps.v, a.c.v, a.c, rows)) return cudaErrorNotSupported;
     constexpr int base = k8_smem_bytes<D, NT, NW>();
     if (!p.split) {
         constexpr auto f = k_kv8_attend_whole<T, E4M3, D, NT, NW>;
         const cudaError_t e = allow_smem<f>(base, a.c.device);
         if (e != cudaSuccess) return e;
-        f<<<p.grid, NW * 32, base, st>>>(a);
+        f<<<p.grid, NW * 32, base, st>>>(a, maps);
         return cudaGetLastError();
     }
     constexpr auto f = k_kv8_attend_split<T, E4M3, D, NT, NW>;
     const int smem = base + (a.c.n_seqs + 1) * 8;
     cudaError_t e = allow_smem<f>(base + (K8_MAX_SPLIT_SEQS + 1) * 8, a.c.device);
     if (e != cudaSuccess) return e;
-    f<<<p.grid, NW * 32, smem, st>>>(a);
+    f<<<p.grid, NW * 32, smem, st>>>(a, maps);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     // the join may become resident while the split kernel runs; it waits for its results
     cudaLaunchConfig_t cfg{};

@@ -22,7 +22,7 @@ namespace qtts {
 
 constexpr int K8_PAGE = 64, K8_BLOCK = 16, K8_RING = 32;
 constexpr int K8_BPP = K8_PAGE / K8_BLOCK;      // blocks per page
-enum : int { K8_BAD_PAGE = 1, K8_BAD_LEN = 2, K8_BAD_ROWS = 4, K8_SHARED_PAGE = 8 };   // status bits
+enum : int { K8_BAD_PAGE = 1, K8_BAD_LEN = 2, K8_BAD_ROWS = 4, K8_SHARED_PAGE = 8, K8_STUCK = 16 };   // status bits
 
 // A sequence's share of a call, checked against the cache: rows [row0, row0 + n)
 // of the packed tensors, its length after them.  Numbers that do not fit set a

@@ -10,6 +10,8 @@
 // The products run on the tensor cores in F16 with F32 sums: codes of both kinds
 // are exact in F16, the scales stay outside in F32.
 #pragma once
+#include <cuda.h>
+
 #include "kv8.cuh"
 
 namespace qtts {
@@ -43,12 +45,16 @@ __device__ __forceinline__ void k8_span(const K8Seq & s, int i, int window, int 
 // is the output, O^T = V^T P^T (16 dims x 8 rows): with one query token a group of
 // G <= 8 heads fills one MMA column tile, where the usual orientation would pad it
 // to 16.  An MMA's inner index may be permuted freely if both operands agree, so a
-// lane copies what it needs straight from the page, in 16-byte words:
-//   K: lane (g, t) = (lane / 4, lane % 4) holds 16 consecutive dims of keys g and g + 8
-//      per 64 dims; word w of them is one k-step (4 dims a lane).
-//   V: the lane holds D / 8 dims (from 16 g on, per 128) of tokens 2t, 2t+1, 2t+8, 2t+9;
-//      dims 2j and 2j+1 of them are rows g and g + 8 of output tile j.
-// So nothing is exchanged or transposed between the page and the MMA.
+// lane reads what it needs from a block's rows as 16-byte words:
+//   K: lane (g, t) = (lane / 4, lane % 4) holds 16 consecutive dims (chunk t of each 64)
+//      of keys k8_key(g) and k8_key(g) + 8; word w of them is one k-step (4 dims a lane).
+//   V: the lane holds D / 8 dims (chunk g of each 128) of the keys of MMA rows 2t, 2t+1
+//      and those + 8; dims 2j and 2j+1 of them are rows g and g + 8 of output tile j.
+// Nothing is exchanged or transposed between the page and the MMA.  The rows lie in
+// shared memory as TMA's 128-byte swizzle leaves them (16-byte chunk ^= row % 8), and
+// k8_key's order spreads both patterns over all banks: eight lanes read chunks t of two
+// keys that differ in bit 2 (K), and chunks g, g ^ 1 of four keys that differ in bits
+// 1 and 2 (V).
 __device__ __forceinline__ uint32_t k8_prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
 // Four codes -> two F16 pairs (bytes 0, 1 and 2, 3).
 template <bool E4M3> __device__ __forceinline__ void k8_f16x4(uint32_t w, uint32_t & lo, uint32_t & hi);
@@ -84,49 +90,33 @@ __device__ __forceinline__ uint32_t k8_transpose(uint32_t x) {   // an 8 x 8 mat
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ void k8_copy16(uint32_t dst, const uint8_t * src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void k8_copy8(uint32_t dst, const uint8_t * src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void k8_copy4(uint32_t dst, const float * src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void k8_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void k8_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ int k8_key(int g) { return g ^ (g & 1) << 2; }   // the key of MMA row g
 
-// A slot of a warp's ring in shared memory: the codes of U blocks, every lane's own
-// words at its own place (word i of lane l at 16 (32 i + l): no bank conflicts, and a
-// lane waits for its own copies only), then the blocks' scales.
+struct K8Maps { CUtensorMap k, v; };             // the pools as [pages * kv heads * 64][D] bytes, boxes of k8_box rows x min(D, 128)
+
+// A slot of a warp's ring in shared memory: the K and the V rows of U blocks (D = 256: in
+// two halves of 128 dims), swizzled.  Beside the ring: the page's scales and a barrier
+// for each slot.
 template <int D, int U> struct K8Slot {
-    static constexpr int k_bytes = D * 16, v_bytes = D * 16, block = k_bytes + v_bytes, s_at = U * block, bytes = s_at + 16;
+    static constexpr int rows = U * K8_BLOCK, row_bytes = D < 128 ? D : 128, half = rows * row_bytes, side = D < 256 ? half : 2 * half, bytes = 2 * side;
 };
-template <int D, int U> __device__ __forceinline__ void k8_fetch(uint32_t slot, const K8AttendArgs & a, int page, int h, int block, int lane) {
-    const int H = a.c.n_kv_heads, g = lane >> 2, t = lane & 3;
-    const int64_t at = k8_code_off(page, h, block * K8_BLOCK, H, D);
-    const uint8_t * k = static_cast<const uint8_t *>(a.c.k) + at + g * D + t * 16;
-    const uint8_t * v = static_cast<const uint8_t *>(a.c.v) + at + 2 * t * D + (D == 64 ? g * 8 : g * 16);
-    const uint32_t ks = slot + lane * 16, vs = slot + K8Slot<D, U>::k_bytes + lane * (D == 64 ? 8 : 16);
+__device__ __forceinline__ void k8_tma(uint32_t dst, const CUtensorMap * map, int x, int y, uint64_t * bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+// One lane: a step's rows and its page's scales into a slot.
+template <int D, int U>
+__device__ __forceinline__ void k8_fetch(uint32_t slot, float * scales, uint64_t * bar, const K8AttendArgs & a, const K8Maps & maps, int page, int h, int block) {
+    using Slot = K8Slot<D, U>;
+    const int H = a.c.n_kv_heads, y = (page * H + h) * K8_PAGE + block * K8_BLOCK;
+    mbar_expect_tx(bar, Slot::bytes + 32);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        constexpr int B = K8Slot<D, U>::block;
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-            k8_copy16(ks + u * B + (2 * c) * 512, k + u * K8_BLOCK * D + c * 64);
-            k8_copy16(ks + u * B + (2 * c + 1) * 512, k + u * K8_BLOCK * D + 8 * D + c * 64);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint8_t * p = v + (u * K8_BLOCK + (i & 1) + (i >> 1) * 8) * D;
-            if constexpr (D == 64) k8_copy8(vs + u * B + i * 256, p);
-            else {
-#pragma unroll
-                for (int c = 0; c < D / 128; ++c) k8_copy16(vs + u * B + (i * (D / 128) + c) * 512, p + c * 128);
-            }
-        }
+    for (int x = 0; x < D; x += 128) {
+        k8_tma(slot + x / 128 * Slot::half, &maps.k, x, y, bar);
+        k8_tma(slot + Slot::side + x / 128 * Slot::half, &maps.v, x, y, bar);
     }
-    if (lane < 2 * U) k8_copy4(slot + K8Slot<D, U>::s_at + lane * 4, (lane & 1 ? a.c.v_scale : a.c.k_scale) + k8_scale_off(page, h, block + (lane >> 1), H));
+    bulk_g2s(scales, a.c.k_scale + k8_scale_off(page, h, 0, H), 16, bar);
+    bulk_g2s(scales + 4, a.c.v_scale + k8_scale_off(page, h, 0, H), 16, bar);
 }
 __device__ __forceinline__ uint4 k8_lds16(uint32_t p) {
     uint4 r;
@@ -213,13 +203,27 @@ struct K8Rows { int lo[2], hi[2]; };              // keys of the lane's rows 8 n
 template <int D, int NT> constexpr int K8_U = D * NT <= 128 ? 2 : 1;
 template <int D, int NT> constexpr int K8_SLOTS = D == 64 ? (NT == 1 ? 3 : 6) : (D == 128 ? (NT == 1 ? 2 : 4) : 2);
 
-// Steps first, first + step, .. < last of U blocks each.
+struct K8Ring { uint32_t ring; float * scales; uint64_t * bar; };   // a warp's own: slots, 8 scales and a barrier for each
+
+// Steps first, first + step, .. < last of U blocks each.  `phase`: each slot's next parity.
 template <bool E4M3, class T, int D, int NT>
 __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (&q)[NT], const float (&fac)[NT][2], const K8Rows (&rows)[NT],
                                           const K8AttendArgs & a, const int32_t * table, int h, int first, int last, int step, int all_lo, int all_hi,
-                                          int any_hi, uint32_t ring, int lane) {
+                                          int any_hi, const K8Maps & maps, const K8Ring & R, uint32_t & phase, int lane) {
     constexpr int S = K8_SLOTS<D, NT>, U = K8_U<D, NT>, KEYS = U * K8_BLOCK, SPP = K8_PAGE / KEYS;
     using Slot = K8Slot<D, U>;
+    // a lane's places in a block: K chunk t of key kr (chunk 4 + t: ^ 64 bytes), V chunk g of keys 2t and vr
+    const int g = lane >> 2, t = lane & 3, kr = k8_key(g), vr = k8_key(2 * t + 1);
+    uint32_t k_at, v_at0, v_at1;
+    if constexpr (D == 64) {   // 64-byte rows, swizzle of 64 bytes: chunk ^= row / 2 % 4
+        k_at = kr * 64 + ((t ^ (kr >> 1 & 3)) << 4);
+        v_at0 = 2 * t * 64 + (((g >> 1) ^ t) << 4) + (g & 1) * 8;
+        v_at1 = vr * 64 + (((g >> 1) ^ (vr >> 1 & 3)) << 4) + (g & 1) * 8;
+    } else {
+        k_at = kr * 128 + ((t ^ kr) << 4);
+        v_at0 = 2 * t * 128 + ((g ^ (2 * t)) << 4);
+        v_at1 = vr * 128 + ((g ^ vr) << 4);
+    }
     const int count = first < last ? (last - first + step - 1) / step : 0;
     // page numbers of the next 64 steps, two to a lane
     auto page_of = [&](int i) { return i < count ? k8_page(table, (first + i * step) / SPP, a.c.n_pages) : -1; };
@@ -232,26 +236,29 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
             const int page = __shfl_sync(0xffffffffu, pg0, i & 31);
             if (page >= 0) {
                 good |= 1u << slot;
-                k8_fetch<D, U>(ring + slot * Slot::bytes, a, page, h, (first + i * step) % SPP * U, lane);
+                if (lane == 0) k8_fetch<D, U>(R.ring + slot * Slot::bytes, R.scales + slot * 8, R.bar + slot, a, maps, page, h, (first + i * step) % SPP * U);
             } else if (lane == 0) k8_flag(a.c.status, K8_BAD_PAGE);
         }
-        k8_commit();
     };
 #pragma unroll
     for (int i = 0; i < S; ++i) fetch(i, i);
     int slot = 0;
     for (int i = 0; i < count; ++i) {
         const int j0 = (first + i * step) * KEYS;   // the step's first key
-        const uint32_t at = ring + slot * Slot::bytes;
-        k8_wait<S - 1>();
-        __syncwarp();                               // the scales are other lanes' copies
-        if (good >> slot & 1) {
+        const uint32_t at = R.ring + slot * Slot::bytes;
+        bool have = good >> slot & 1;
+        if (have) {
+            have = __all_sync(0xffffffffu, mbar_wait(R.bar + slot, phase >> slot & 1));
+            phase ^= 1u << slot;
+            if (!have && lane == 0) k8_flag(a.c.status, K8_STUCK);
+        }
+        if (have) {
             float ks[U], vs[U], s[U][NT][4];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint2 sc = k8_lds8(at + Slot::s_at + u * 8);
-                ks[u] = __uint_as_float(sc.x);
-                vs[u] = __uint_as_float(sc.y);
+                const int block = (first + i * step) % SPP * U + u;
+                ks[u] = R.scales[slot * 8 + block];
+                vs[u] = R.scales[slot * 8 + 4 + block];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -261,8 +268,8 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
             for (int c = 0; c < D / 64; ++c)
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const uint32_t kp = at + u * Slot::block + lane * 16;
-                    const uint4 x = k8_lds16(kp + (2 * c) * 512), y = k8_lds16(kp + (2 * c + 1) * 512);
+                    const uint32_t kp = at + (c >> 1) * Slot::half + u * K8_BLOCK * Slot::row_bytes + (c & 1 ? k_at ^ 64 : k_at);
+                    const uint4 x = k8_lds16(kp), y = k8_lds16(kp + 8 * Slot::row_bytes);
                     const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
@@ -283,7 +290,7 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
                     for (int e = 0; e < 4; ++e) {
                         s[u][nt][e] *= fac[nt][e & 1] * ks[u];
                         if (!whole) {
-                            const int j = j0 + u * K8_BLOCK + (lane >> 2) + (e >> 1) * 8;
+                            const int j = j0 + u * K8_BLOCK + kr + (e >> 1) * 8;
                             if (j < rows[nt].lo[e & 1] || j >= rows[nt].hi[e & 1]) s[u][nt][e] = -INFINITY;
                         }
                     }
@@ -337,29 +344,30 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
                         st.l[nt][i & 1] += hidden ? 0.0f : x;
                         e[i] = hidden ? 0.0f : x * rv;
                     }
-                    p[u][nt][0] = k8_transpose(k8_pack(e[0], e[1]));
+                    p[u][nt][0] = k8_transpose(k8_pack(e[0], e[1]));   // rows of the transpose: keys 2t, 2t + 1 in MMA order
                     p[u][nt][1] = k8_transpose(k8_pack(e[2], e[3]));
                 }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 // rows of the page past the sequence's end may hold anything
-                const int beyond = whole ? K8_BLOCK : any_hi - j0 - u * K8_BLOCK - 2 * (lane & 3);
-                const uint32_t vp = at + u * Slot::block + Slot::k_bytes + lane * (D == 64 ? 8 : 16);
+                const int beyond = any_hi - j0 - u * K8_BLOCK;
+                const uint32_t vp = at + Slot::side + u * K8_BLOCK * Slot::row_bytes;
 #pragma unroll
                 for (int c = 0; c < (D + 127) / 128; ++c) {
                     uint32_t v[4][4];
                     constexpr int W = D == 64 ? 2 : 4;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
+                        const uint32_t p = vp + c * Slot::half + (i & 1 ? v_at1 : v_at0) + (i >> 1) * 8 * Slot::row_bytes;
                         if constexpr (D == 64) {
-                            const uint2 x = k8_lds8(vp + i * 256);
+                            const uint2 x = k8_lds8(p);
                             v[i][0] = x.x; v[i][1] = x.y;
                         } else {
-                            const uint4 x = k8_lds16(vp + (i * (D / 128) + c) * 512);
+                            const uint4 x = k8_lds16(p);
                             v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
                         }
-                        if (!whole && (i & 1) + (i >> 1) * 8 >= beyond)
+                        if (!whole && (i & 1 ? vr : 2 * t) + (i >> 1) * 8 >= beyond)
 #pragma unroll
                             for (int w = 0; w < W; ++w) v[i][w] = 0;
                     }
@@ -381,10 +389,16 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
             }
         }
         __syncwarp();                               // the slot has been read
+        if (!have && (good >> slot & 1)) {          // a copy that never came: no more of them, and none in flight at the end
+            for (int o = 1; o < S; ++o) {
+                const int other = (slot + o) % S;
+                if (good >> other & 1) { mbar_wait(R.bar + other, phase >> other & 1); phase ^= 1u << other; }
+            }
+            break;
+        }
         fetch(i + S, slot);
         slot = slot + 1 == S ? 0 : slot + 1;
     }
-    k8_wait<0>();
 }
 
 // What a CTA of the split kernel leaves of an item it has only a part of:
@@ -408,7 +422,8 @@ template <class T> __device__ __forceinline__ void k8_write_row(const K8AttendAr
 // warps take its blocks in turn, their states are joined in shared memory in
 // warp order.  `dst` null: the item is complete and goes to out and lse.
 template <class T, bool E4M3, int D, int NT, int NW>
-__device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq & s, int b, int h, int tile, int pg0, int pg1, float * dst, float * smem) {
+__device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Maps & maps, const K8Seq & s, int b, int h, int tile, int pg0, int pg1, float * dst,
+                                           const K8Ring & ring, uint32_t & phase, float * smem) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3;
     const int G = a.n_heads / a.c.n_kv_heads, R = s.n * G, r0 = tile * 8 * NT;
     K8Q<T, D> q[NT];
@@ -445,7 +460,7 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq &
     constexpr int KEYS = K8_U<D, NT> * K8_BLOCK;
     const int X0 = max(pg0 * (K8_PAGE / KEYS), lo / KEYS), X1 = min(pg1 * (K8_PAGE / KEYS), (hi1 + KEYS - 1) / KEYS);
     k8_blocks<E4M3, T, D, NT>(st, q, fac, rows, a, a.table + (int64_t) b * a.c.max_pages, h, X0 + warp, X1, NW, lo1, hi, hi1,
-                              smem_u32(smem) + warp * K8_SLOTS<D, NT> * K8Slot<D, K8_U<D, NT>>::bytes, lane);
+                              maps, ring, phase, lane);
     // join: rows' sums over lanes, then the warps through the shared memory that held the rings
     __syncthreads();
     float * sm = smem, * sl = smem + NW * 8 * NT, * so = smem + 2 * NW * 8 * NT;   // [NW][8 NT] twice, [NW][8 NT][D + 4]
@@ -486,11 +501,33 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Seq &
             if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = l == 0.0f ? -INFINITY : (m - K8_LIFT + log2f(l)) * 0.693147180559945309417f;
         }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next segment's copies write where the join wrote
     __syncthreads();
 }
+// Shared memory: the warps' rings, which the join uses too (a multiple of 1 KB, on a 1 KB
+// boundary for the swizzle), their slots' scales and barriers.
+template <int D, int NT, int NW> __host__ __device__ constexpr int k8_ring_bytes() {
+    const int rings = NW * K8_SLOTS<D, NT> * K8Slot<D, K8_U<D, NT>>::bytes, join = (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4;
+    return ((rings > join ? rings : join) + 1023) / 1024 * 1024;
+}
 template <int D, int NT, int NW> __host__ __device__ constexpr int k8_smem_bytes() {
-    return (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4 > NW * K8_SLOTS<D, NT> * K8Slot<D, K8_U<D, NT>>::bytes ? (2 * NW * 8 * NT + NW * 8 * NT * (D + 4)) * 4
-                                                                                               : NW * K8_SLOTS<D, NT> * K8Slot<D, K8_U<D, NT>>::bytes;
+    return 1024 + k8_ring_bytes<D, NT, NW>() + NW * K8_SLOTS<D, NT> * (32 + 8);
+}
+extern __shared__ __align__(1024) uint8_t k8_dyn[];
+template <int D, int NT, int NW> __device__ __forceinline__ uint8_t * k8_ring(K8Ring & r) {
+    constexpr int S = K8_SLOTS<D, NT>;
+    const int warp = threadIdx.x >> 5;
+    uint8_t * base = k8_dyn + (-(int) smem_u32(k8_dyn) & 1023);
+    r.ring = smem_u32(base) + warp * S * K8Slot<D, K8_U<D, NT>>::bytes;
+    r.scales = reinterpret_cast<float *>(base + k8_ring_bytes<D, NT, NW>()) + warp * S * 8;
+    r.bar = reinterpret_cast<uint64_t *>(base + k8_ring_bytes<D, NT, NW>() + NW * S * 32) + warp * S;
+    if ((threadIdx.x & 31) == 0) {
+        for (int i = 0; i < S; ++i) mbar_init(r.bar + i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    return base;
 }
 
 // CTAs of 4 warps that are resident together, by their registers.
@@ -498,8 +535,7 @@ __host__ __device__ constexpr int k8_ctas_per_sm(int dim, int nt) { return dim *
 
 // One CTA per (sequence, kv head, row tile).
 template <class T, bool E4M3, int D, int NT, int NW>
-__global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_whole(K8AttendArgs a) {
-    extern __shared__ __align__(16) float k8_smem[];
+__global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_whole(K8AttendArgs a, const __grid_constant__ K8Maps maps) {
     const int H = a.c.n_kv_heads, G = a.n_heads / H;
     const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles % H, b = blockIdx.x / a.tiles / H;
     const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
@@ -507,7 +543,10 @@ __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_w
     if (tile * 8 * NT >= s.n * G) return;
     int pg0, pg1;
     k8_pages(s, a.window, pg0, pg1);
-    k8_segment<T, E4M3, D, NT, NW>(a, s, b, h, tile, pg0, pg1, nullptr, k8_smem);
+    K8Ring ring;
+    float * smem = reinterpret_cast<float *>(k8_ring<D, NT, NW>(ring));
+    uint32_t phase = 0;
+    k8_segment<T, E4M3, D, NT, NW>(a, maps, s, b, h, tile, pg0, pg1, nullptr, ring, phase, smem);
 }
 
 // Split along the cache.  All (sequence, kv head, row tile) items laid end to end are
@@ -550,11 +589,13 @@ __device__ __forceinline__ long long k8_chunk(long long total, int ctas) {
 }
 
 template <class T, bool E4M3, int D, int NT, int NW>
-__global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_split(K8AttendArgs a) {
-    extern __shared__ __align__(16) float k8_smem[];
+__global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_split(K8AttendArgs a, const __grid_constant__ K8Maps maps) {
     __shared__ long long s_carry[NW];
     pdl_trigger();
-    long long * at = reinterpret_cast<long long *>(k8_smem + k8_smem_bytes<D, NT, NW>() / 4);
+    K8Ring ring;
+    float * smem = reinterpret_cast<float *>(k8_ring<D, NT, NW>(ring));
+    uint32_t phase = 0;
+    long long * at = reinterpret_cast<long long *>(reinterpret_cast<uint8_t *>(smem) + k8_smem_bytes<D, NT, NW>() - 1024);
     k8_line<NT, NW * 32>(a, at, s_carry);
     const long long total = at[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
     long long pos = blockIdx.x * chunk;
@@ -573,7 +614,7 @@ __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_s
         const int p1 = (int)(np - p0 < end - pos ? np : p0 + (end - pos));
         const bool whole = p0 == 0 && p1 == np;
         float * dst = whole ? nullptr : a.part + ((long long) blockIdx.x * 2 + (first ? 0 : 1)) * K8Part<D, NT>::floats;
-        k8_segment<T, E4M3, D, NT, NW>(a, s, lo, item / tiles, item % tiles, pg0 + p0, pg0 + p1, dst, k8_smem);
+        k8_segment<T, E4M3, D, NT, NW>(a, maps, s, lo, item / tiles, item % tiles, pg0 + p0, pg0 + p1, dst, ring, phase, smem);
         pos += p1 - p0;
         first = false;
     }

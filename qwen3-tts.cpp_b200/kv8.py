@@ -19,7 +19,7 @@ from .engine import lib
 PAGE, BLOCK, RING = 64, 16, 32
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 STATUS = {1: "a page number outside the pool", 2: "a length outside the page table", 4: "rows outside the call's tensors",
-          8: "a destination page that is in use"}
+          8: "a destination page that is in use", 16: "a copy that did not arrive in time"}
 
 
 class RopeArgs(C.Structure):
