@@ -120,7 +120,7 @@ template <class F> void by_cache(const qtts_kv8 & c, F f) {
 // How an attention call runs.  Rows of a (sequence, kv head) come in tiles of 8 nt;
 // one CTA takes a tile's whole range, or, with few tiles over a long cache, the
 // ranges are split evenly over the GPU.
-struct K8Plan { int nt, tiles, split, ctas; int64_t part_bytes; unsigned grid; };
+struct K8Plan { int nt, tiles, split, ctas, part_rows; int64_t line_bytes, part_bytes; unsigned grid; };   // workspace: line, parts, lse
 constexpr int SMS = 148, NW = 4;
 bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     const int64_t R = (int64_t) p.max_q * (p.n_heads / c.n_kv_heads);
@@ -130,7 +130,9 @@ bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     o->tiles = (int) tiles;
     o->split = c.max_pages > 8 && R <= 64 && c.n_seqs <= K8_MAX_SPLIT_SEQS;
     o->ctas = SMS * k8_ctas_per_sm(c.head_dim, o->nt);
-    o->part_bytes = o->split ? (int64_t) o->ctas * 2 * 8 * o->nt * (c.head_dim + 2) * 4 : 0;
+    o->part_rows = (int)(R < 8 * o->nt ? R : 8 * o->nt);
+    o->line_bytes = o->split ? ((int64_t) c.n_seqs + 2) / 2 * 16 : 0;
+    o->part_bytes = o->split ? (int64_t) o->ctas * 2 * o->part_rows * (c.head_dim + 4) * 4 : 0;
     o->grid = (unsigned)(o->split ? o->ctas : items);
     return true;
 }
@@ -333,7 +335,7 @@ int64_t qtts_kv8_attend_ws(const qtts_kv8 * c, const qtts_kv8_attend * p) {
     if (bad_cache(c) || !p || p->n_rows < 0 || p->n_heads < 1) return -1;
     K8Plan plan;
     if (p->n_heads % c->n_kv_heads || p->max_q < 0 || !attend_plan(*c, *p, &plan)) return -1;
-    return plan.part_bytes + (p->weight_out && !p->lse ? ((int64_t) p->n_rows * p->n_heads * 4 + 15) / 16 * 16 : 0);
+    return plan.line_bytes + plan.part_bytes + (p->weight_out && !p->lse ? ((int64_t) p->n_rows * p->n_heads * 4 + 15) / 16 * 16 : 0);
 }
 
 int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * p, void * stream) {
@@ -363,9 +365,10 @@ int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * p, void *
     if (p->weight_out && !grid_of((int64_t) c->n_seqs * c->n_kv_heads * c->max_pages * K8_PAGE, 4, &gw)) return refuse(who, "too much work for one call");
     K8Plan plan;
     if (!attend_plan(*c, *p, &plan)) return refuse(who, "too much work for one call");
-    if (p->weight_out && !a.lse) a.lse = reinterpret_cast<float *>(static_cast<uint8_t *>(p->ws) + plan.part_bytes);
-    a.part = static_cast<float *>(p->ws);
-    a.tiles = plan.tiles; a.ctas = plan.ctas;
+    if (p->weight_out && !a.lse) a.lse = reinterpret_cast<float *>(static_cast<uint8_t *>(p->ws) + plan.line_bytes + plan.part_bytes);
+    a.line = static_cast<long long *>(p->ws);
+    a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(p->ws) + plan.line_bytes);
+    a.tiles = plan.tiles; a.ctas = plan.ctas; a.part_rows = plan.part_rows;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t err = cudaSuccess;
     by_cache(*c, [&](auto t, auto e, auto d) {

@@ -11,6 +11,7 @@
 // are exact in F16, the scales stay outside in F32.
 #pragma once
 #include <cuda.h>
+#include <type_traits>
 
 #include "kv8.cuh"
 
@@ -28,9 +29,11 @@ struct K8AttendArgs {
     const float * w_in;                        // [n_seqs][H][w_stride] or null
     float * w_out;
     int64_t w_stride;
-    float * part;                              // partial results (split kernel), see K8Split
+    long long * line;                          // split kernel: [n_seqs + 1] pages of work before each sequence
+    float * part;                              // and its partial results
     int tiles;                                 // row tiles of one (sequence, kv head)
     int ctas;                                  // CTAs of the split kernel
+    int part_rows;                             // rows of a partial result
 };
 
 // Keys [lo, hi) of row i of a sequence.
@@ -280,113 +283,118 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
                         for (int nt = 0; nt < NT; ++nt) k8_mma(s[u][nt], a0, a1, a2, a3, q[nt].x[4 * c + w][0], q[nt].x[4 * c + w][1]);
                     }
                 }
-            const bool whole = j0 >= all_lo && j0 + KEYS <= all_hi;   // every row sees every key
-            bool up = false;
+            // The rest of the step, twice: `whole` where every row sees every key, else with masks.
+            auto finish = [&](auto whole_c) {
+                constexpr bool whole = decltype(whole_c)::value;
+                bool up = false;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[u][nt][e] *= fac[nt][e & 1] * ks[u];
-                        if (!whole) {
-                            const int j = j0 + u * K8_BLOCK + kr + (e >> 1) * 8;
-                            if (j < rows[nt].lo[e & 1] || j >= rows[nt].hi[e & 1]) s[u][nt][e] = -INFINITY;
+                        for (int e = 0; e < 4; ++e) {
+                            s[u][nt][e] *= fac[nt][e & 1] * ks[u];
+                            if constexpr (!whole) {
+                                const int j = j0 + u * K8_BLOCK + kr + (e >> 1) * 8;
+                                if (j < rows[nt].lo[e & 1] || j >= rows[nt].hi[e & 1]) s[u][nt][e] = -INFINITY;
+                            }
+                        }
+                        up |= fmaxf(s[u][nt][0], s[u][nt][2]) > st.m[nt][0] + K8_SLACK || fmaxf(s[u][nt][1], s[u][nt][3]) > st.m[nt][1] + K8_SLACK;
+                    }
+                if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            float m = fmaxf(s[0][nt][r], s[0][nt][r + 2]);
+#pragma unroll
+                            for (int u = 1; u < U; ++u) m = fmaxf(m, fmaxf(s[u][nt][r], s[u][nt][r + 2]));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                            m = fmaxf(m, st.m[nt][r]);
+                            const float f = m == st.m[nt][r] ? 1.0f : k8_exp2(st.m[nt][r] - m);
+                            st.m[nt][r] = m;
+                            st.l[nt][r] *= f;
+#pragma unroll
+                            for (int j = 0; j < D / 16; ++j) { st.o[nt][j][r] *= f; st.o[nt][j][r + 2] *= f; }
+                        }
+                }
+                float top = vs[0];
+#pragma unroll
+                for (int u = 1; u < U; ++u) top = fmaxf(top, vs[u]);
+                if (top > st.unit * K8_UNIT_SLACK) {    // the same for the whole warp
+                    const float f = st.unit / top;
+                    st.unit = top;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) st.o[nt][j][e] *= f;
+                }
+                const float inv = __fdividef(1.0f, st.unit);
+                uint32_t p[U][NT][2];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float rv = vs[u] * inv;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float e[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = k8_exp2(s[u][nt][i] - (st.m[nt][i & 1] - K8_LIFT));
+                            // a key that a row does not see adds nothing, even before the row has seen any or if a scale is NaN
+                            const bool hidden = !whole && s[u][nt][i] == -INFINITY;
+                            st.l[nt][i & 1] += hidden ? 0.0f : x;
+                            e[i] = hidden ? 0.0f : x * rv;
+                        }
+                        p[u][nt][0] = k8_transpose(k8_pack(e[0], e[1]));   // rows of the transpose: keys 2t, 2t + 1 in MMA order
+                        p[u][nt][1] = k8_transpose(k8_pack(e[2], e[3]));
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    // rows of the page past the sequence's end may hold anything
+                    const int beyond = any_hi - j0 - u * K8_BLOCK;
+                    const uint32_t vp = at + Slot::side + u * K8_BLOCK * Slot::row_bytes;
+#pragma unroll
+                    for (int c = 0; c < (D + 127) / 128; ++c) {
+                        uint32_t v[4][4];
+                        constexpr int W = D == 64 ? 2 : 4;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t p = vp + c * Slot::half + (i & 1 ? v_at1 : v_at0) + (i >> 1) * 8 * Slot::row_bytes;
+                            if constexpr (D == 64) {
+                                const uint2 x = k8_lds8(p);
+                                v[i][0] = x.x; v[i][1] = x.y;
+                            } else {
+                                const uint4 x = k8_lds16(p);
+                                v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
+                            }
+                            if (!whole && (i & 1 ? vr : 2 * t) + (i >> 1) * 8 >= beyond)
+#pragma unroll
+                                for (int w = 0; w < W; ++w) v[i][w] = 0;
+                        }
+#pragma unroll
+                        for (int w = 0; w < W; ++w) {
+                            uint32_t a0[2], a1[2], a2[2], a3[2];
+                            // tokens' bytes side by side: [x0 y0 x1 y1], [x2 y2 x3 y3]
+                            k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x5140), a0[0], a1[0]);
+                            k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x7362), a0[1], a1[1]);
+                            k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x5140), a2[0], a3[0]);
+                            k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x7362), a2[1], a3[1]);
+#pragma unroll
+                            for (int o = 0; o < 2; ++o)
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+                                    k8_mma(st.o[nt][c * 8 + 2 * w + o], a0[o], a1[o], a2[o], a3[o], p[u][nt][0], p[u][nt][1]);
                         }
                     }
-                    up |= fmaxf(s[u][nt][0], s[u][nt][2]) > st.m[nt][0] + K8_SLACK || fmaxf(s[u][nt][1], s[u][nt][3]) > st.m[nt][1] + K8_SLACK;
                 }
-            if (__any_sync(0xffffffffu, up)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float m = fmaxf(s[0][nt][r], s[0][nt][r + 2]);
-#pragma unroll
-                        for (int u = 1; u < U; ++u) m = fmaxf(m, fmaxf(s[u][nt][r], s[u][nt][r + 2]));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                        m = fmaxf(m, st.m[nt][r]);
-                        const float f = m == st.m[nt][r] ? 1.0f : k8_exp2(st.m[nt][r] - m);
-                        st.m[nt][r] = m;
-                        st.l[nt][r] *= f;
-#pragma unroll
-                        for (int j = 0; j < D / 16; ++j) { st.o[nt][j][r] *= f; st.o[nt][j][r + 2] *= f; }
-                    }
-            }
-            float top = vs[0];
-#pragma unroll
-            for (int u = 1; u < U; ++u) top = fmaxf(top, vs[u]);
-            if (top > st.unit * K8_UNIT_SLACK) {    // the same for the whole warp
-                const float f = st.unit / top;
-                st.unit = top;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) st.o[nt][j][e] *= f;
-            }
-            const float inv = __fdividef(1.0f, st.unit);
-            uint32_t p[U][NT][2];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const float rv = vs[u] * inv;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float e[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = k8_exp2(s[u][nt][i] - (st.m[nt][i & 1] - K8_LIFT));
-                        // a key that a row does not see adds nothing, even before the row has seen any or if a scale is NaN
-                        const bool hidden = !whole && s[u][nt][i] == -INFINITY;
-                        st.l[nt][i & 1] += hidden ? 0.0f : x;
-                        e[i] = hidden ? 0.0f : x * rv;
-                    }
-                    p[u][nt][0] = k8_transpose(k8_pack(e[0], e[1]));   // rows of the transpose: keys 2t, 2t + 1 in MMA order
-                    p[u][nt][1] = k8_transpose(k8_pack(e[2], e[3]));
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                // rows of the page past the sequence's end may hold anything
-                const int beyond = any_hi - j0 - u * K8_BLOCK;
-                const uint32_t vp = at + Slot::side + u * K8_BLOCK * Slot::row_bytes;
-#pragma unroll
-                for (int c = 0; c < (D + 127) / 128; ++c) {
-                    uint32_t v[4][4];
-                    constexpr int W = D == 64 ? 2 : 4;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t p = vp + c * Slot::half + (i & 1 ? v_at1 : v_at0) + (i >> 1) * 8 * Slot::row_bytes;
-                        if constexpr (D == 64) {
-                            const uint2 x = k8_lds8(p);
-                            v[i][0] = x.x; v[i][1] = x.y;
-                        } else {
-                            const uint4 x = k8_lds16(p);
-                            v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
-                        }
-                        if (!whole && (i & 1 ? vr : 2 * t) + (i >> 1) * 8 >= beyond)
-#pragma unroll
-                            for (int w = 0; w < W; ++w) v[i][w] = 0;
-                    }
-#pragma unroll
-                    for (int w = 0; w < W; ++w) {
-                        uint32_t a0[2], a1[2], a2[2], a3[2];
-                        // tokens' bytes side by side: [x0 y0 x1 y1], [x2 y2 x3 y3]
-                        k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x5140), a0[0], a1[0]);
-                        k8_f16x4<E4M3>(k8_prmt(v[0][w], v[1][w], 0x7362), a0[1], a1[1]);
-                        k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x5140), a2[0], a3[0]);
-                        k8_f16x4<E4M3>(k8_prmt(v[2][w], v[3][w], 0x7362), a2[1], a3[1]);
-#pragma unroll
-                        for (int o = 0; o < 2; ++o)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                k8_mma(st.o[nt][c * 8 + 2 * w + o], a0[o], a1[o], a2[o], a3[o], p[u][nt][0], p[u][nt][1]);
-                    }
-                }
-            }
+            };
+            if (j0 >= all_lo && j0 + KEYS <= all_hi) finish(std::true_type{});
+            else finish(std::false_type{});
         }
         __syncwarp();                               // the slot has been read
         if (!have && (good >> slot & 1)) {          // a copy that never came: no more of them, and none in flight at the end
@@ -401,10 +409,6 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
     }
 }
 
-// What a CTA of the split kernel leaves of an item it has only a part of:
-// [CTA][first or last segment][8 NT rows] of m, l and [8 NT rows][D] of o.
-template <int D, int NT> struct K8Part { static constexpr int floats = 8 * NT * (D + 2); };
-
 // Pages [pg0, pg1) of a sequence that any of its rows sees.
 __device__ __forceinline__ void k8_pages(const K8Seq & s, int window, int & pg0, int & pg1) {
     int lo, hi;
@@ -418,13 +422,12 @@ template <class T> __device__ __forceinline__ void k8_write_row(const K8AttendAr
     static_cast<T *>(a.out)[row * a.o_row + hq * a.o_head + d] = T(o * inv);
 }
 
-// One segment (pages of one (sequence, kv head, row tile)) by the whole CTA: the
-// warps take its blocks in turn, their states are joined in shared memory in
-// warp order.  `dst` null: the item is complete and goes to out and lse.
-template <class T, bool E4M3, int D, int NT, int NW>
-__device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Maps & maps, const K8Seq & s, int b, int h, int tile, int pg0, int pg1, float * dst,
-                                           const K8Ring & ring, uint32_t & phase, float * smem) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3;
+// One warp: its share (steps first, first + step, ..) of pages [pg0, pg1) of one
+// (sequence, kv head, row tile).
+template <class T, bool E4M3, int D, int NT>
+__device__ __forceinline__ void k8_run(K8State<D, NT> & st, const K8AttendArgs & a, const K8Maps & maps, const K8Seq & s, int b, int h, int tile, int pg0, int pg1,
+                                       int first, int step, const K8Ring & ring, uint32_t & phase) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
     const int G = a.n_heads / a.c.n_kv_heads, R = s.n * G, r0 = tile * 8 * NT;
     K8Q<T, D> q[NT];
     float fac[NT][2];
@@ -446,7 +449,6 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Maps 
     int lo, hi, lo1, hi1;
     k8_span(s, r0 / G, a.window, lo, hi);
     k8_span(s, min(r0 + 8 * NT - 1, R - 1) / G, a.window, lo1, hi1);
-    K8State<D, NT> st;
     st.unit = K8_UNIT_MIN;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -459,9 +461,24 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Maps 
         }
     constexpr int KEYS = K8_U<D, NT> * K8_BLOCK;
     const int X0 = max(pg0 * (K8_PAGE / KEYS), lo / KEYS), X1 = min(pg1 * (K8_PAGE / KEYS), (hi1 + KEYS - 1) / KEYS);
-    k8_blocks<E4M3, T, D, NT>(st, q, fac, rows, a, a.table + (int64_t) b * a.c.max_pages, h, X0 + warp, X1, NW, lo1, hi, hi1,
+    k8_blocks<E4M3, T, D, NT>(st, q, fac, rows, a, a.table + (int64_t) b * a.c.max_pages, h, X0 + first, X1, step, lo1, hi, hi1,
                               maps, ring, phase, lane);
-    // join: rows' sums over lanes, then the warps through the shared memory that held the rings
+}
+// The sum of a row's weights over the lanes that hold its keys.
+__device__ __forceinline__ float k8_row_sum(float l) {
+    l += __shfl_xor_sync(0xffffffffu, l, 4);
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    return l + __shfl_xor_sync(0xffffffffu, l, 16);
+}
+__device__ __forceinline__ float k8_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m - K8_LIFT + log2f(l)) * 0.693147180559945309417f; }
+
+// The warps' states of a CTA that shared an item or a part of it, joined in warp order
+// through the shared memory that held the rings: to out and lse (part null), or
+// unnormalised to part [part_rows][D + 4] (o, m, l).
+template <class T, int D, int NT, int NW>
+__device__ __forceinline__ void k8_join_warps(const K8State<D, NT> & st, const K8AttendArgs & a, const K8Seq & s, int h, int tile, float * part, float * smem) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3;
+    const int G = a.n_heads / a.c.n_kv_heads, R = s.n * G, r0 = tile * 8 * NT;
     __syncthreads();
     float * sm = smem, * sl = smem + NW * 8 * NT, * so = smem + 2 * NW * 8 * NT;   // [NW][8 NT] twice, [NW][8 NT][D + 4]
     constexpr int LD = D + 4;
@@ -469,10 +486,7 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Maps 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float l = st.l[nt][i];
-            l += __shfl_xor_sync(0xffffffffu, l, 4);
-            l += __shfl_xor_sync(0xffffffffu, l, 8);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const float l = k8_row_sum(st.l[nt][i]);
             const int r = nt * 8 + 2 * t + i;
             if (lane < 4) { sm[warp * 8 * NT + r] = st.m[nt][i]; sl[warp * 8 * NT + r] = l; }
 #pragma unroll
@@ -492,13 +506,13 @@ __device__ __forceinline__ void k8_segment(const K8AttendArgs & a, const K8Maps 
             l = fmaf(sl[w * 8 * NT + r], f, l);
             o = fmaf(so[(w * 8 * NT + r) * LD + d], f, o);
         }
-        if (dst) {
-            if (d == 0) { dst[r] = m; dst[8 * NT + r] = l; }
-            dst[16 * NT + r * D + d] = o;
+        if (part) {
+            part[r * (D + 4) + d] = o;
+            if (d == 0) { part[r * (D + 4) + D] = m; part[r * (D + 4) + D + 1] = l; }
         } else {
             const int row = s.row0 + rr / G, hq = h * G + rr % G;
             k8_write_row<T>(a, row, hq, d, o, l == 0.0f ? 0.0f : 1.0f / l);
-            if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = l == 0.0f ? -INFINITY : (m - K8_LIFT + log2f(l)) * 0.693147180559945309417f;
+            if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = k8_lse(m, l);
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next segment's copies write where the join wrote
@@ -546,15 +560,19 @@ __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_w
     K8Ring ring;
     float * smem = reinterpret_cast<float *>(k8_ring<D, NT, NW>(ring));
     uint32_t phase = 0;
-    k8_segment<T, E4M3, D, NT, NW>(a, maps, s, b, h, tile, pg0, pg1, nullptr, ring, phase, smem);
+    K8State<D, NT> st;
+    k8_run<T, E4M3, D, NT>(st, a, maps, s, b, h, tile, pg0, pg1, threadIdx.x >> 5, NW, ring, phase);
+    k8_join_warps<T, D, NT, NW>(st, a, s, h, tile, nullptr, smem);
 }
 
 // Split along the cache.  All (sequence, kv head, row tile) items laid end to end are
-// T pages of work; CTA c takes pages [c * chunk, (c + 1) * chunk) of that line, so
-// ragged lengths balance to a page whatever they are.  An item that a CTA holds
-// whole is finished there; parts (a CTA's first and last segment at most) go to
-// `part` and are joined by k_kv8_join.
-constexpr int K8_MAX_SPLIT_SEQS = 1024, K8_MIN_PAGES = 4;
+// a line of pages; CTA c takes pages [c * chunk, (c + 1) * chunk) of it, so ragged
+// lengths balance to a page whatever they are.  An item that a CTA holds whole is
+// finished there; parts (a CTA's first and last segment at most) go to `part` and are
+// joined by k_kv8_join.  (A range for each warp of its own measured 61 and 72 us where
+// this takes 59 and 60, at 32 sequences of 4,400 and two of 131,072: four times the
+// parts to join.)
+constexpr int K8_MAX_SPLIT_SEQS = 1024;
 // Prefix sums over the sequences of their pages of work in `at` [n_seqs + 1].
 template <int NT, int THREADS>
 __device__ __forceinline__ void k8_line(const K8AttendArgs & a, long long * at, long long * s_carry) {
@@ -583,9 +601,10 @@ __device__ __forceinline__ void k8_line(const K8AttendArgs & a, long long * at, 
     }
     __syncthreads();
 }
+// Pages of a CTA: at least 4, so that each warp has some.
 __device__ __forceinline__ long long k8_chunk(long long total, int ctas) {
     const long long c = (total + ctas - 1) / ctas;
-    return c < K8_MIN_PAGES ? K8_MIN_PAGES : c;
+    return c < 4 ? 4 : c;
 }
 
 template <class T, bool E4M3, int D, int NT, int NW>
@@ -593,10 +612,12 @@ __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_s
     __shared__ long long s_carry[NW];
     pdl_trigger();
     K8Ring ring;
-    float * smem = reinterpret_cast<float *>(k8_ring<D, NT, NW>(ring));
+    uint8_t * base = k8_ring<D, NT, NW>(ring);
     uint32_t phase = 0;
-    long long * at = reinterpret_cast<long long *>(reinterpret_cast<uint8_t *>(smem) + k8_smem_bytes<D, NT, NW>() - 1024);
+    long long * at = reinterpret_cast<long long *>(base + k8_smem_bytes<D, NT, NW>() - 1024);
     k8_line<NT, NW * 32>(a, at, s_carry);
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i <= a.c.n_seqs; i += NW * 32) a.line[i] = at[i];
     const long long total = at[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
     long long pos = blockIdx.x * chunk;
     const long long end = pos + chunk < total ? pos + chunk : total;
@@ -612,9 +633,10 @@ __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_s
         const long long in = pos - at[lo];
         const int item = (int)(in / np), p0 = (int)(in % np);
         const int p1 = (int)(np - p0 < end - pos ? np : p0 + (end - pos));
-        const bool whole = p0 == 0 && p1 == np;
-        float * dst = whole ? nullptr : a.part + ((long long) blockIdx.x * 2 + (first ? 0 : 1)) * K8Part<D, NT>::floats;
-        k8_segment<T, E4M3, D, NT, NW>(a, maps, s, lo, item / tiles, item % tiles, pg0 + p0, pg0 + p1, dst, ring, phase, smem);
+        float * part = p0 == 0 && p1 == np ? nullptr : a.part + ((long long) blockIdx.x * 2 + (first ? 0 : 1)) * a.part_rows * (D + 4);
+        K8State<D, NT> st;
+        k8_run<T, E4M3, D, NT>(st, a, maps, s, lo, item / tiles, item % tiles, pg0 + p0, pg0 + p1, threadIdx.x >> 5, NW, ring, phase);
+        k8_join_warps<T, D, NT, NW>(st, a, s, item / tiles, item % tiles, part, reinterpret_cast<float *>(base));
         pos += p1 - p0;
         first = false;
     }
@@ -626,20 +648,18 @@ __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_s
 constexpr int K8_JOIN_WARPS = 8;
 template <class T, int D, int NT>
 __global__ void __launch_bounds__(K8_JOIN_WARPS * 32) k_kv8_join(K8AttendArgs a) {
-    __shared__ long long at[K8_MAX_SPLIT_SEQS + 1], s_carry[K8_JOIN_WARPS];
     __shared__ float s_m[K8_JOIN_WARPS], s_l[K8_JOIN_WARPS], s_o[K8_JOIN_WARPS][D];
     constexpr int V = D / 32;
     const int H = a.c.n_kv_heads, G = a.n_heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rr = blockIdx.x % (a.max_q * G), h = blockIdx.x / (a.max_q * G) % H, b = blockIdx.x / (a.max_q * G) / H;
-    k8_line<NT, K8_JOIN_WARPS * 32>(a, at, s_carry);
-    pdl_wait();                                     // every CTA, so that the join does not end before the split kernel
-    const long long total = at[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
     const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
-    if (rr >= s.n * G) return;
     int pg0, pg1;
     k8_pages(s, a.window, pg0, pg1);
+    pdl_wait();                                     // every CTA, so that the join does not end before the split kernel
+    if (rr >= s.n * G) return;
+    const long long total = a.line[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
     const int np = pg1 - pg0, tiles = (s.n * G + 8 * NT - 1) / (8 * NT), tile = rr / (8 * NT), r = rr % (8 * NT);
-    const long long p0 = at[b] + (long long)(h * tiles + tile) * np, p1 = p0 + np;
+    const long long p0 = a.line[b] + (long long)(h * tiles + tile) * np, p1 = p0 + np;
     const int c0 = (int)(p0 / chunk), c1 = np ? (int)((p1 - 1) / chunk) : c0 - 1;
     if (c0 == c1) return;                           // one CTA had all of it
     float m = -INFINITY, l = 0.0f, o[V];
@@ -647,10 +667,10 @@ __global__ void __launch_bounds__(K8_JOIN_WARPS * 32) k_kv8_join(K8AttendArgs a)
     for (int e = 0; e < V; ++e) o[e] = 0.0f;
 #pragma unroll 4
     for (int c = c0 + warp; c <= c1; c += K8_JOIN_WARPS) {
-        const float * p = a.part + ((long long) c * 2 + (c == c0 && p0 > c * chunk ? 1 : 0)) * K8Part<D, NT>::floats;
+        const float * p = a.part + (((long long) c * 2 + (c == c0 && p0 > c * chunk ? 1 : 0)) * a.part_rows + r) * (D + 4);
         struct alignas(V * 4 > 16 ? 16 : V * 4) Vec { float x[V]; };
-        const Vec x = *reinterpret_cast<const Vec *>(p + 16 * NT + r * D + lane * V);
-        const float mc = p[r], lc = p[8 * NT + r], mn = fmaxf(m, mc);
+        const Vec x = *reinterpret_cast<const Vec *>(p + lane * V);
+        const float mc = p[D], lc = p[D + 1], mn = fmaxf(m, mc);
         const float f = m == mn ? 1.0f : k8_exp2(m - mn), fc = mc == mn ? 1.0f : k8_exp2(mc - mn);
         m = mn;
         l = l * f + lc * fc;
@@ -674,7 +694,7 @@ __global__ void __launch_bounds__(K8_JOIN_WARPS * 32) k_kv8_join(K8AttendArgs a)
     }
     const int row = s.row0 + rr / G, hq = h * G + rr % G;
     k8_write_row<T>(a, row, hq, d, O, L == 0.0f ? 0.0f : 1.0f / L);
-    if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = L == 0.0f ? -INFINITY : (M - K8_LIFT + log2f(L)) * 0.693147180559945309417f;
+    if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = k8_lse(M, L);
 }
 
 // Accumulated weights, plain: one warp per (sequence, kv head, key), rows and heads in order.
