@@ -128,13 +128,29 @@ bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     const int64_t tiles = (R + 8 * o->nt - 1) / (8 * o->nt), items = tiles * c.n_kv_heads * c.n_seqs;
     if (items > 0x7fffffff) return false;
     o->tiles = (int) tiles;
-    o->split = c.max_pages > 8 && R <= 64 && c.n_seqs <= K8_MAX_SPLIT_SEQS;
+    o->split = c.max_pages > 8 && R <= 64 && c.n_seqs <= K8_MAX_SPLIT_SEQS && items * c.max_pages < 0x40000000;
     o->ctas = SMS * k8_ctas_per_sm(c.head_dim, o->nt);
     o->part_rows = (int)(R < 8 * o->nt ? R : 8 * o->nt);
-    o->line_bytes = o->split ? ((int64_t) c.n_seqs + 2) / 2 * 16 : 0;
+    o->line_bytes = o->split ? ((int64_t) c.n_seqs + 4) / 4 * 16 : 0;
     o->part_bytes = o->split ? (int64_t) o->ctas * 2 * o->part_rows * (c.head_dim + 4) * 4 : 0;
     o->grid = (unsigned)(o->split ? o->ctas : items);
     return true;
+}
+// Programmatic dependent launch: the kernel may be set up while its predecessor runs,
+// and waits for it (pdl_wait) before it reads or writes memory.
+template <class... P, class... A>
+cudaError_t pdl_go(void (*f)(P...), unsigned grid, int block, int smem, cudaStream_t st, A &&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, f, std::forward<A>(args)...);
 }
 // The shared memory limit of a kernel, raised once per device.
 template <auto F> cudaError_t allow_smem(int bytes, int device) {
@@ -173,26 +189,15 @@ cudaError_t attend_launch(const K8AttendArgs & a, const K8Plan & p, cudaStream_t
         constexpr auto f = k_kv8_attend_whole<T, E4M3, D, NT, NW>;
         const cudaError_t e = allow_smem<f>(base, a.c.device);
         if (e != cudaSuccess) return e;
-        f<<<p.grid, NW * 32, base, st>>>(a, maps);
-        return cudaGetLastError();
+        return pdl_go(f, p.grid, NW * 32, base, st, a, maps);
     }
     constexpr auto f = k_kv8_attend_split<T, E4M3, D, NT, NW>;
-    const int smem = base + (a.c.n_seqs + 1) * 8;
-    cudaError_t e = allow_smem<f>(base + (K8_MAX_SPLIT_SEQS + 1) * 8, a.c.device);
+    const int smem = base + (a.c.n_seqs + 1) * 4;
+    cudaError_t e = allow_smem<f>(base + (K8_MAX_SPLIT_SEQS + 1) * 4, a.c.device);
     if (e != cudaSuccess) return e;
-    f<<<p.grid, NW * 32, smem, st>>>(a, maps);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    // the join may become resident while the split kernel runs; it waits for its results
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((int64_t) a.c.n_seqs * a.c.n_kv_heads * a.max_q * (a.n_heads / a.c.n_kv_heads)));
-    cfg.blockDim = dim3(K8_JOIN_WARPS * 32);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_kv8_join<T, D, NT>, a);
+    if ((e = pdl_go(f, p.grid, NW * 32, smem, st, a, maps)) != cudaSuccess) return e;
+    return pdl_go(k_kv8_join<T, D, NT>, (unsigned)((int64_t) a.c.n_seqs * a.c.n_kv_heads * a.max_q * (a.n_heads / a.c.n_kv_heads)), K8_JOIN_WARPS * 32,
+                  0, st, a);
 }
 
 }  // namespace
@@ -366,7 +371,7 @@ int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * p, void *
     K8Plan plan;
     if (!attend_plan(*c, *p, &plan)) return refuse(who, "too much work for one call");
     if (p->weight_out && !a.lse) a.lse = reinterpret_cast<float *>(static_cast<uint8_t *>(p->ws) + plan.line_bytes + plan.part_bytes);
-    a.line = static_cast<long long *>(p->ws);
+    a.line = static_cast<int *>(p->ws);
     a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(p->ws) + plan.line_bytes);
     a.tiles = plan.tiles; a.ctas = plan.ctas; a.part_rows = plan.part_rows;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -29,7 +29,7 @@ struct K8AttendArgs {
     const float * w_in;                        // [n_seqs][H][w_stride] or null
     float * w_out;
     int64_t w_stride;
-    long long * line;                          // split kernel: [n_seqs + 1] pages of work before each sequence
+    int * line;                                // split kernel: [n_seqs + 1] pages of work before each sequence
     float * part;                              // and its partial results
     int tiles;                                 // row tiles of one (sequence, kv head)
     int ctas;                                  // CTAs of the split kernel
@@ -488,6 +488,7 @@ __device__ __forceinline__ void k8_join_warps(const K8State<D, NT> & st, const K
         for (int i = 0; i < 2; ++i) {
             const float l = k8_row_sum(st.l[nt][i]);
             const int r = nt * 8 + 2 * t + i;
+            if (r0 + r >= R) continue;
             if (lane < 4) { sm[warp * 8 * NT + r] = st.m[nt][i]; sl[warp * 8 * NT + r] = l; }
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
@@ -552,6 +553,8 @@ template <class T, bool E4M3, int D, int NT, int NW>
 __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_whole(K8AttendArgs a, const __grid_constant__ K8Maps maps) {
     const int H = a.c.n_kv_heads, G = a.n_heads / H;
     const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles % H, b = blockIdx.x / a.tiles / H;
+    pdl_trigger();
+    pdl_wait();
     const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
     if (threadIdx.x == 0 && h == 0 && tile == 0) k8_flag(a.c.status, s.status);
     if (tile * 8 * NT >= s.n * G) return;
@@ -575,26 +578,26 @@ __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_w
 constexpr int K8_MAX_SPLIT_SEQS = 1024;
 // Prefix sums over the sequences of their pages of work in `at` [n_seqs + 1].
 template <int NT, int THREADS>
-__device__ __forceinline__ void k8_line(const K8AttendArgs & a, long long * at, long long * s_carry) {
+__device__ __forceinline__ void k8_line(const K8AttendArgs & a, int * at, int * s_carry) {
     const int H = a.c.n_kv_heads, G = a.n_heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) { at[0] = 0; }
-    long long base = 0;
+    int base = 0;
     for (int b0 = 0; b0 < a.c.n_seqs; b0 += THREADS) {
         const int b = b0 + threadIdx.x;
-        long long w = 0;
+        int w = 0;
         if (b < a.c.n_seqs) {
             const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
             if (blockIdx.x == 0) k8_flag(a.c.status, s.status);
             int pg0, pg1;
             k8_pages(s, a.window, pg0, pg1);
-            w = (long long)(pg1 - pg0) * H * ((s.n * G + 8 * NT - 1) / (8 * NT));
+            w = (pg1 - pg0) * H * ((s.n * G + 8 * NT - 1) / (8 * NT));
         }
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, w, o); if (lane >= o) w += y; }
+        for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, w, o); if (lane >= o) w += y; }
         __syncthreads();
         if (lane == 31) s_carry[warp] = w;
         __syncthreads();
-        long long before = base;
+        int before = base;
         for (int i = 0; i < warp; ++i) before += s_carry[i];
         if (b < a.c.n_seqs) at[b + 1] = before + w;
         for (int i = 0; i < THREADS / 32; ++i) base += s_carry[i];
@@ -602,25 +605,26 @@ __device__ __forceinline__ void k8_line(const K8AttendArgs & a, long long * at, 
     __syncthreads();
 }
 // Pages of a CTA: at least 4, so that each warp has some.
-__device__ __forceinline__ long long k8_chunk(long long total, int ctas) {
-    const long long c = (total + ctas - 1) / ctas;
+__device__ __forceinline__ int k8_chunk(int total, int ctas) {
+    const int c = (total + ctas - 1) / ctas;
     return c < 4 ? 4 : c;
 }
 
 template <class T, bool E4M3, int D, int NT, int NW>
 __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_split(K8AttendArgs a, const __grid_constant__ K8Maps maps) {
-    __shared__ long long s_carry[NW];
+    __shared__ int s_carry[NW];
     pdl_trigger();
+    pdl_wait();
     K8Ring ring;
     uint8_t * base = k8_ring<D, NT, NW>(ring);
     uint32_t phase = 0;
-    long long * at = reinterpret_cast<long long *>(base + k8_smem_bytes<D, NT, NW>() - 1024);
+    int * at = reinterpret_cast<int *>(base + k8_smem_bytes<D, NT, NW>() - 1024);
     k8_line<NT, NW * 32>(a, at, s_carry);
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i <= a.c.n_seqs; i += NW * 32) a.line[i] = at[i];
-    const long long total = at[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
-    long long pos = blockIdx.x * chunk;
-    const long long end = pos + chunk < total ? pos + chunk : total;
+    const int total = at[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
+    int pos = min(total, (int) blockIdx.x * chunk);
+    const int end = min(total, pos + chunk);
     const int G = a.n_heads / a.c.n_kv_heads;
     bool first = true;
     while (pos < end) {
@@ -630,10 +634,8 @@ __global__ void __launch_bounds__(NW * 32, k8_ctas_per_sm(D, NT)) k_kv8_attend_s
         int pg0, pg1;
         k8_pages(s, a.window, pg0, pg1);
         const int np = pg1 - pg0, tiles = (s.n * G + 8 * NT - 1) / (8 * NT);
-        const long long in = pos - at[lo];
-        const int item = (int)(in / np), p0 = (int)(in % np);
-        const int p1 = (int)(np - p0 < end - pos ? np : p0 + (end - pos));
-        float * part = p0 == 0 && p1 == np ? nullptr : a.part + ((long long) blockIdx.x * 2 + (first ? 0 : 1)) * a.part_rows * (D + 4);
+        const int item = (pos - at[lo]) / np, p0 = (pos - at[lo]) % np, p1 = min(np, p0 + end - pos);
+        float * part = p0 == 0 && p1 == np ? nullptr : a.part + ((int64_t) blockIdx.x * 2 + (first ? 0 : 1)) * a.part_rows * (D + 4);
         K8State<D, NT> st;
         k8_run<T, E4M3, D, NT>(st, a, maps, s, lo, item / tiles, item % tiles, pg0 + p0, pg0 + p1, threadIdx.x >> 5, NW, ring, phase);
         k8_join_warps<T, D, NT, NW>(st, a, s, item / tiles, item % tiles, part, reinterpret_cast<float *>(base));
@@ -652,22 +654,23 @@ __global__ void __launch_bounds__(K8_JOIN_WARPS * 32) k_kv8_join(K8AttendArgs a)
     constexpr int V = D / 32;
     const int H = a.c.n_kv_heads, G = a.n_heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rr = blockIdx.x % (a.max_q * G), h = blockIdx.x / (a.max_q * G) % H, b = blockIdx.x / (a.max_q * G) / H;
+    pdl_trigger();
+    pdl_wait();                                     // every CTA, so that the join does not end before the split kernel
     const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
     int pg0, pg1;
     k8_pages(s, a.window, pg0, pg1);
-    pdl_wait();                                     // every CTA, so that the join does not end before the split kernel
     if (rr >= s.n * G) return;
-    const long long total = a.line[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
+    const int total = a.line[a.c.n_seqs], chunk = k8_chunk(total, a.ctas);
     const int np = pg1 - pg0, tiles = (s.n * G + 8 * NT - 1) / (8 * NT), tile = rr / (8 * NT), r = rr % (8 * NT);
-    const long long p0 = a.line[b] + (long long)(h * tiles + tile) * np, p1 = p0 + np;
-    const int c0 = (int)(p0 / chunk), c1 = np ? (int)((p1 - 1) / chunk) : c0 - 1;
+    const int p0 = a.line[b] + (h * tiles + tile) * np, p1 = p0 + np;
+    const int c0 = p0 / chunk, c1 = np ? (p1 - 1) / chunk : c0 - 1;
     if (c0 == c1) return;                           // one CTA had all of it
     float m = -INFINITY, l = 0.0f, o[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] = 0.0f;
 #pragma unroll 4
     for (int c = c0 + warp; c <= c1; c += K8_JOIN_WARPS) {
-        const float * p = a.part + (((long long) c * 2 + (c == c0 && p0 > c * chunk ? 1 : 0)) * a.part_rows + r) * (D + 4);
+        const float * p = a.part + ((int64_t)(c * 2 + (c == c0 && p0 > c * chunk ? 1 : 0)) * a.part_rows + r) * (D + 4);
         struct alignas(V * 4 > 16 ? 16 : V * 4) Vec { float x[V]; };
         const Vec x = *reinterpret_cast<const Vec *>(p + lane * V);
         const float mc = p[D], lc = p[D + 1], mn = fmaxf(m, mc);
