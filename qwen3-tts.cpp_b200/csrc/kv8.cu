@@ -22,10 +22,7 @@ int32_t refuse(const char * who, const char * why) {
     set_op_error(buf);
     return 0;
 }
-int32_t launched(const char * who) {
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? 1 : refuse(who, cudaGetErrorString(e));
-}
+int32_t result(const char * who, cudaError_t e) { return e == cudaSuccess ? 1 : refuse(who, cudaGetErrorString(e)); }
 
 // The call's device for the launches, the caller's afterwards.
 struct OnDevice {
@@ -67,38 +64,54 @@ bool grid_of(int64_t units, int per, unsigned * g) {
     return true;
 }
 
+// Programmatic dependent launch: the kernel may be set up while its predecessor runs,
+// and waits for it (pdl_wait) before it reads or writes memory.
+template <class... P, class... A>
+cudaError_t pdl_go(void (*f)(P...), dim3 grid, int block, int smem, cudaStream_t st, A &&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, f, std::forward<A>(args)...);
+}
+template <class T, int MODE> cudaError_t rope_go(const RopeArgs & a, unsigned g, int lanes, cudaStream_t st) {
+    if (lanes == 8) return pdl_go(k_rope<T, 8, MODE>, g, ROPE_WARPS * 32, 0, st, a);
+    if (lanes == 16) return pdl_go(k_rope<T, 16, MODE>, g, ROPE_WARPS * 32, 0, st, a);
+    return pdl_go(k_rope<T, 32, MODE>, g, ROPE_WARPS * 32, 0, st, a);
+}
 template <class T> int32_t rope_launch(const RopeArgs & a, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
     const uintptr_t all = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.q_out) |
                           reinterpret_cast<uintptr_t>(a.k_out);
     const int64_t strides = a.qs_row | a.qs_head | a.qo_row | a.qo_head | (a.k ? a.ks_row | a.ks_head | a.ko_row | a.ko_head : 0);
-    const int V = a.dim / 32;
-    const bool vec = (a.dim == 64 || a.dim == 128 || a.dim == 256) && sizeof(T) * V <= 16 && all % (sizeof(T) * V) == 0 && strides % V == 0;
-    if (!vec) {
-        const int64_t units = (int64_t) a.rows * (a.q_heads + a.k_heads) * (a.dim - a.rot / 2);
-        const int64_t g = (units + 255) / 256;
-        k_rope_any<T><<<(unsigned)(g < 148 * 64 ? g : 148 * 64), 256, 0, st>>>(a);
-        return launched("qtts_op_rope");
+    const int lanes = a.dim / V;
+    cudaError_t e;
+    if (a.dim % V || (lanes != 8 && lanes != 16 && lanes != 32) || all % 16 || strides % V) {
+        const int64_t units = (int64_t) a.rows * (a.q_heads + a.k_heads) * (a.dim - a.rot / 2), g = (units + 255) / 256;
+        e = pdl_go(k_rope_any<T>, (unsigned)(g < 148 * 64 ? g : 148 * 64), 256, 0, st, a);
+    } else {
+        RopeArgs b = a;
+        // many rows: a warp takes all heads of a row, so its angles are computed once; few rows: one step's heads each, so
+        // that the warps cover the GPU
+        const int heads = a.q_heads + a.k_heads, step = 32 / lanes;
+        const int64_t warps = 148 * 32, per = ((int64_t) a.rows * heads + warps - 1) / warps;
+        b.heads_per_warp = (int)(per >= heads ? heads : (per + step - 1) / step * step);
+        b.chunks = (heads + b.heads_per_warp - 1) / b.heads_per_warp;
+        unsigned g;
+        if (!grid_of((int64_t) a.rows * b.chunks, ROPE_WARPS, &g)) return refuse("qtts_op_rope", "too many rows");
+        if (a.interleaved) e = rope_go<T, ROPE_PAIR>(b, g, lanes, st);
+        else if (a.rot / 2 % V == 0) e = rope_go<T, ROPE_WORD>(b, g, lanes, st);
+        else e = rope_go<T, ROPE_VALUE>(b, g, lanes, st);
     }
-    RopeArgs b = a;
-    const int heads = a.q_heads + a.k_heads;
-    // few rows: one head per warp; many: a warp computes its row's angles once for all heads
-    const int64_t want = 148 * 64;
-    int per = (int)(((int64_t) a.rows * heads + want - 1) / want);
-    b.heads_per_warp = per < 1 ? 1 : (per > heads ? heads : per);
-    b.chunks = (heads + b.heads_per_warp - 1) / b.heads_per_warp;
-    unsigned g;
-    if (!grid_of((int64_t) a.rows * b.chunks, ROPE_WARPS, &g)) return refuse("qtts_op_rope", "too many rows");
-    if (V == 2) k_rope<T, 2><<<g, ROPE_WARPS * 32, 0, st>>>(b);
-    else if (V == 4) k_rope<T, 4><<<g, ROPE_WARPS * 32, 0, st>>>(b);
-    else if constexpr (sizeof(T) == 2) k_rope<T, 8><<<g, ROPE_WARPS * 32, 0, st>>>(b);
-    return launched("qtts_op_rope");
+    return result("qtts_op_rope", e);
 }
 
-template <class T, bool E4M3, int D>
-void append_launch(const K8Args & a, bool vec, unsigned g, cudaStream_t st) {
-    if (vec) k_kv8_append<T, E4M3, D, true><<<g, K8_WARPS * 32, 0, st>>>(a);
-    else k_kv8_append<T, E4M3, D, false><<<g, K8_WARPS * 32, 0, st>>>(a);
-}
 // calls f.template operator()<T, E4M3, D>() for the cache's row type, code and head size
 template <class F> void by_cache(const qtts_kv8 & c, F f) {
     auto by_dim = [&](auto t, auto e) {
@@ -135,22 +148,6 @@ bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     o->part_bytes = o->split ? (int64_t) o->ctas * 2 * o->part_rows * (c.head_dim + 4) * 4 : 0;
     o->grid = (unsigned)(o->split ? o->ctas : items);
     return true;
-}
-// Programmatic dependent launch: the kernel may be set up while its predecessor runs,
-// and waits for it (pdl_wait) before it reads or writes memory.
-template <class... P, class... A>
-cudaError_t pdl_go(void (*f)(P...), unsigned grid, int block, int smem, cudaStream_t st, A &&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, f, std::forward<A>(args)...);
 }
 // The shared memory limit of a kernel, raised once per device.
 template <auto F> cudaError_t allow_smem(int bytes, int device) {
@@ -302,10 +299,15 @@ int32_t qtts_op_kv8_append(const qtts_kv8 * c, const int32_t * table, const int3
     a.blocks = (int)(((int64_t) max_new + 2 * K8_BLOCK - 2) / K8_BLOCK);   // a run of max_new rows touches at most this many blocks
     const bool vec = aligned(k, 16) && aligned(v, 16) && (k_row | k_head | v_row | v_head) % 8 == 0;
     unsigned g;
-    if (!grid_of((int64_t) c->n_seqs * a.blocks * c->n_kv_heads * 2, K8_WARPS, &g)) return refuse(who, "too many rows");
+    if (!grid_of((int64_t) a.blocks * c->n_kv_heads * 2, K8_WARPS, &g) || g > 0x7fffffff / K8_WARPS) return refuse(who, "too many rows");
+    const dim3 grid(g, (unsigned) c->n_seqs);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    by_cache(*c, [&](auto t, auto e, auto d) { append_launch<decltype(t), decltype(e)::value, decltype(d)::value>(a, vec, g, st); });
-    return launched(who);
+    cudaError_t err = cudaSuccess;
+    by_cache(*c, [&](auto t, auto e, auto d) {
+        if (vec) err = pdl_go(k_kv8_append<decltype(t), decltype(e)::value, decltype(d)::value, true>, grid, K8_WARPS * 32, 0, st, a);
+        else err = pdl_go(k_kv8_append<decltype(t), decltype(e)::value, decltype(d)::value, false>, grid, K8_WARPS * 32, 0, st, a);
+    });
+    return result(who, err);
 }
 
 int32_t qtts_op_kv8_read(const qtts_kv8 * c, const int32_t * table, const int32_t * begin, const int32_t * cu, int32_t out_type,
@@ -321,19 +323,16 @@ int32_t qtts_op_kv8_read(const qtts_kv8 * c, const int32_t * table, const int32_
     OnDevice on(c->device);
     if (!on.ok) return refuse(who, "device");
     K8ReadArgs a{};
-    a.c = *c; a.table = table; a.begin = begin; a.cu = cu; a.n_rows = n_rows; a.max_n = max_rows; a.out_type = out_type; a.k = k; a.v = v;
-    const int64_t gx = ((int64_t) max_rows * c->n_kv_heads * (c->head_dim / 8) + 255) / 256;
-    const dim3 g((unsigned)(gx < (1 << 20) ? gx : (1 << 20)), (unsigned) c->n_seqs);
+    a.c = *c; a.table = table; a.begin = begin; a.cu = cu; a.n_rows = n_rows; a.max_n = max_rows; a.k = k; a.v = v;
+    const int per_row = c->n_kv_heads * (c->head_dim / 16);
+    a.rows_per_cta = per_row >= 512 ? 1 : 512 / per_row;
+    const dim3 grid((unsigned)((max_rows + (int64_t) a.rows_per_cta - 1) / a.rows_per_cta), (unsigned) c->n_seqs);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto go = [&](auto t) {
         using T = decltype(t);
-        if (c->code) k_kv8_read<T, true><<<g, 256, 0, st>>>(a);
-        else k_kv8_read<T, false><<<g, 256, 0, st>>>(a);
+        return c->code ? pdl_go(k_kv8_read<T, true>, grid, 256, 0, st, a) : pdl_go(k_kv8_read<T, false>, grid, 256, 0, st, a);
     };
-    if (out_type == 0) go(0.0f);
-    else if (out_type == 1) go(__half{});
-    else go(__nv_bfloat16{});
-    return launched(who);
+    return result(who, out_type == 0 ? go(0.0f) : (out_type == 1 ? go(__half{}) : go(__nv_bfloat16{})));
 }
 
 int64_t qtts_kv8_attend_ws(const qtts_kv8 * c, const qtts_kv8_attend * p) {
@@ -366,8 +365,6 @@ int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * p, void *
     a.q_row = p->q_row; a.q_head = p->q_head; a.o_row = p->o_row; a.o_head = p->o_head;
     a.n_rows = p->n_rows; a.max_q = p->max_q; a.n_heads = p->n_heads; a.window = p->window; a.scale = p->scale; a.lse = p->lse;
     a.w_in = p->weight_in; a.w_out = p->weight_out; a.w_stride = p->weight_stride;
-    unsigned gw = 0;
-    if (p->weight_out && !grid_of((int64_t) c->n_seqs * c->n_kv_heads * c->max_pages * K8_PAGE, 4, &gw)) return refuse(who, "too much work for one call");
     K8Plan plan;
     if (!attend_plan(*c, *p, &plan)) return refuse(who, "too much work for one call");
     if (p->weight_out && !a.lse) a.lse = reinterpret_cast<float *>(static_cast<uint8_t *>(p->ws) + plan.line_bytes + plan.part_bytes);
@@ -385,10 +382,13 @@ int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * p, void *
             else if (plan.nt == 2) err = attend_launch<T, E, D, 2>(a, plan, st);
             else if constexpr (D < 256) err = attend_launch<T, E, D, 4>(a, plan, st);
         }
-        if (p->weight_out) k_kv8_weigh_plain<T, E, D><<<gw, 128, 0, st>>>(a, a.lse);
+        if (p->weight_out && err == cudaSuccess) {
+            constexpr int keys = K8_WEIGH_W<D> * K8_BLOCK * K8_WEIGH_WARPS;
+            const dim3 grid((unsigned)(((int64_t) c->max_pages * K8_PAGE + keys - 1) / keys), (unsigned) c->n_kv_heads, (unsigned) c->n_seqs);
+            err = pdl_go(k_kv8_weigh<T, E, D>, grid, K8_WEIGH_WARPS * 32, 0, st, a);
+        }
     });
-    if (err != cudaSuccess) return refuse(who, cudaGetErrorString(err));
-    return launched(who);
+    return result(who, err);
 }
 
 int32_t qtts_op_kv8_evict(const qtts_kv8 * c, const int32_t * table, const int32_t * lens, const int32_t * dst_table,
@@ -409,14 +409,19 @@ int32_t qtts_op_kv8_evict(const qtts_kv8 * c, const int32_t * table, const int32
     a.c = *c; a.table = table; a.lens = lens; a.dst_table = dst_table; a.dst_pages = dst_pages; a.weight = weight; a.w_stride = weight_stride;
     a.budget = budget; a.sinks = sinks; a.recent = recent; a.lens_out = lens_out; a.keep = keep; a.weight_out = weight_out;
     unsigned g;
-    if (!grid_of((int64_t) c->n_seqs * (budget / K8_BLOCK) * c->n_kv_heads * 2, K8_WARPS, &g)) return refuse(who, "too much work for one call");
+    if (!grid_of((int64_t)(budget / K8_BLOCK) * c->n_kv_heads * 2, K8_WARPS, &g)) return refuse(who, "too much work for one call");
+    const dim3 grid(g, (unsigned) c->n_seqs);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    k_kv8_select<<<(unsigned)(c->n_seqs * c->n_kv_heads), 1024, 0, st>>>(a);
-    by_cache(*c, [&](auto t, auto e, auto d) {
-        (void) t;
-        k_kv8_move<decltype(e)::value, decltype(d)::value><<<g, K8_WARPS * 32, 0, st>>>(a);
-    });
-    return launched(who);
+    const int64_t cap = (int64_t) c->max_pages * K8_PAGE;
+    const int room = cap < K8_SEL_KEYS ? (int) cap : K8_SEL_KEYS;
+    cudaError_t err = allow_smem<k_kv8_select>(K8_SEL_KEYS * 4, c->device);
+    if (err == cudaSuccess) err = pdl_go(k_kv8_select, (unsigned)(c->n_seqs * c->n_kv_heads), K8_SEL_THREADS, room * 4, st, a, room);
+    if (err == cudaSuccess)
+        by_cache(*c, [&](auto t, auto e, auto d) {
+            (void) t;
+            err = pdl_go(k_kv8_move<decltype(e)::value, decltype(d)::value>, grid, K8_WARPS * 32, 0, st, a);
+        });
+    return result(who, err);
 }
 
 }  // extern "C"

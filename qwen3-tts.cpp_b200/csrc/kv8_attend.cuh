@@ -58,23 +58,6 @@ __device__ __forceinline__ void k8_span(const K8Seq & s, int i, int window, int 
 // k8_key's order spreads both patterns over all banks: eight lanes read chunks t of two
 // keys that differ in bit 2 (K), and chunks g, g ^ 1 of four keys that differ in bits
 // 1 and 2 (V).
-__device__ __forceinline__ uint32_t k8_prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
-// Four codes -> two F16 pairs (bytes 0, 1 and 2, 3).
-template <bool E4M3> __device__ __forceinline__ void k8_f16x4(uint32_t w, uint32_t & lo, uint32_t & hi);
-template <> __device__ __forceinline__ void k8_f16x4<false>(uint32_t w, uint32_t & lo, uint32_t & hi) {
-    // byte u = code + 128 as the low mantissa bits of 1024: 1024 + u - 1152 = code, exactly
-    w ^= 0x80808080u;
-    lo = k8_prmt(w, 0x64646464u, 0x4140);
-    hi = k8_prmt(w, 0x64646464u, 0x4342);
-    const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    __half2 a = __hsub2(*reinterpret_cast<__half2 *>(&lo), off), b = __hsub2(*reinterpret_cast<__half2 *>(&hi), off);
-    lo = *reinterpret_cast<uint32_t *>(&a);
-    hi = *reinterpret_cast<uint32_t *>(&b);
-}
-template <> __device__ __forceinline__ void k8_f16x4<true>(uint32_t w, uint32_t & lo, uint32_t & hi) {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-        : "=r"(lo), "=r"(hi) : "r"(w));
-}
 __device__ __forceinline__ void k8_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -700,39 +683,104 @@ __global__ void __launch_bounds__(K8_JOIN_WARPS * 32) k_kv8_join(K8AttendArgs a)
     if (d == 0 && a.lse) a.lse[(int64_t) row * a.n_heads + hq] = k8_lse(M, L);
 }
 
-// Accumulated weights, plain: one warp per (sequence, kv head, key), rows and heads in order.
+// ---- accumulated weights -----------------------------------------------------
+// weight_out = weight_in + each key's weights over the rows and the head group.  A warp
+// owns W blocks of keys of one (sequence, kv head): their K rows as F16 fragments in
+// registers, straight from the page; it goes over the rows eight at a time, recomputes
+// the scores as the attention does and adds exp(s - lse) in row order, so the sum's
+// order is fixed and nothing is exchanged but four lanes at the end.  Reads K (D bytes
+// a key) and 8 bytes of weights; bound by memory for single tokens.
+template <int D> constexpr int K8_WEIGH_W = D == 256 ? 1 : 2;
+constexpr int K8_WEIGH_WARPS = 4;
 template <class T, bool E4M3, int D>
-__global__ void __launch_bounds__(128) k_kv8_weigh_plain(K8AttendArgs a, const float * lse) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31, H = a.c.n_kv_heads, G = a.n_heads / H, cap = a.c.max_pages * K8_PAGE;
-    const int64_t unit = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int j = (int)(unit % cap), h = (int)(unit / cap % H);
-    const int64_t b = unit / cap / H;
-    if (b >= a.c.n_seqs) return;
-    const K8Seq s = k8_seq((int) b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
-    if (j >= s.len) return;
-    const int page = k8_page(a.table + b * a.c.max_pages, j / K8_PAGE, a.c.n_pages);
-    const int64_t wa = (b * H + h) * a.w_stride + j;
-    float w = 0.0f;
-    if (page >= 0) {
-        const int64_t at = k8_code_off(page, h, j % K8_PAGE, H, D) + lane * V;
-        const float sc = a.c.k_scale[k8_scale_off(page, h, j % K8_PAGE / K8_BLOCK, H)];
-        for (int i = 0; i < s.n; ++i) {
-            int lo, hi;
-            k8_span(s, i, a.window, lo, hi);
-            if (j < lo || j >= hi) continue;
-            for (int g = 0; g < G; ++g) {
-                const int row = s.row0 + i, hq = h * G + g;
-                const T * q = static_cast<const T *>(a.q) + row * a.q_row + hq * a.q_head + lane * V;
-                float d = 0.0f;
+__global__ void __launch_bounds__(K8_WEIGH_WARPS * 32) k_kv8_weigh(K8AttendArgs a) {
+    constexpr int W = K8_WEIGH_W<D>, KEYS = W * K8_BLOCK;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, H = a.c.n_kv_heads, G = a.n_heads / H;
+    const int h = blockIdx.y, b = blockIdx.z, j0 = (blockIdx.x * K8_WEIGH_WARPS + (threadIdx.x >> 5)) * KEYS;
+    pdl_trigger();
+    pdl_wait();
+    const K8Seq s = k8_seq(b, a.lens, a.cu, a.c.max_pages, a.n_rows, a.max_q, false);
+    if (j0 >= s.len) return;
+    const int page = k8_page(a.table + (int64_t) b * a.c.max_pages, j0 / K8_PAGE, a.c.n_pages);
+    const float * wi = a.w_in + ((int64_t) b * H + h) * a.w_stride + j0;
+    float * wo = a.w_out + ((int64_t) b * H + h) * a.w_stride + j0;
+    float w[W][2], old[W][2];
 #pragma unroll
-                for (int e = 0; e < V; ++e) d = fmaf((float) q[e], Code8<E4M3>::value(static_cast<const uint8_t *>(a.c.k)[at + e]), d);
-                d = warp_sum(d) * sc * a.scale;
-                w += expf(d - lse[(int64_t) row * a.n_heads + hq]);
+    for (int u = 0; u < W; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int j = u * K8_BLOCK + i * 8 + g;
+            w[u][i] = 0.0f;
+            old[u][i] = t == 0 && j0 + j < s.len ? wi[j] : 0.0f;
+        }
+    if (page >= 0 && s.n > 0) {
+        uint4 raw[W][2][D / 64];
+        float ks[W];
+#pragma unroll
+        for (int u = 0; u < W; ++u) {
+            const int block = j0 % K8_PAGE / K8_BLOCK + u;
+            const uint8_t * k = static_cast<const uint8_t *>(a.c.k) + k8_code_off(page, h, block * K8_BLOCK + g, H, D) + t * 16;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                raw[u][0][c] = ld_stream(k + c * 64);
+                raw[u][1][c] = ld_stream(k + 8 * D + c * 64);
+            }
+            ks[u] = a.c.k_scale[k8_scale_off(page, h, block, H)];
+        }
+        const int R = s.n * G;
+        for (int r0 = 0; r0 < R; r0 += 8) {
+            int lo[2], hi[2], lo0, hi0, lo1, hi1;
+            k8_span(s, r0 / G, a.window, lo0, hi0);
+            k8_span(s, min(r0 + 7, R - 1) / G, a.window, lo1, hi1);
+            if (hi1 <= j0 || lo0 >= j0 + KEYS) continue;         // no row of these sees a key of ours
+            K8Q<T, D> q;
+            const int r = r0 + g;
+            const bool real = r < R;
+            const float back = k8_load_q<T, D>(q, static_cast<const T *>(a.q) + (real ? (s.row0 + r / G) * a.q_row + (h * G + r % G) * a.q_head : 0), lane, real) *
+                               (a.scale * 1.44269504088896340736f);
+            float fac[2], lse[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                fac[i] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * i);
+                const int rr = r0 + 2 * t + i;
+                k8_span(s, min(rr, R - 1) / G, a.window, lo[i], hi[i]);
+                if (rr >= R) hi[i] = 0;                           // rows of padding see nothing
+                lse[i] = rr < R ? a.lse[(int64_t)(s.row0 + rr / G) * a.n_heads + h * G + rr % G] * 1.44269504088896340736f : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < W; ++u) {
+                float c4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c) {
+                    const uint32_t xw[4] = {raw[u][0][c].x, raw[u][0][c].y, raw[u][0][c].z, raw[u][0][c].w};
+                    const uint32_t yw[4] = {raw[u][1][c].x, raw[u][1][c].y, raw[u][1][c].z, raw[u][1][c].w};
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        uint32_t a0, a1, a2, a3;
+                        k8_f16x4<E4M3>(xw[v], a0, a2);
+                        k8_f16x4<E4M3>(yw[v], a1, a3);
+                        k8_mma(c4, a0, a1, a2, a3, q.x[4 * c + v][0], q.x[4 * c + v][1]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = j0 + u * K8_BLOCK + (e >> 1) * 8 + g;
+                    const float p = k8_exp2(c4[e] * (fac[e & 1] * ks[u]) - lse[e & 1]);
+                    w[u][e >> 1] += j >= lo[e & 1] && j < hi[e & 1] ? p : 0.0f;
+                }
             }
         }
-    }
-    if (lane == 0) a.w_out[wa] = a.w_in[wa] + w;
+    } else if (page < 0 && lane == 0) k8_flag(a.c.status, K8_BAD_PAGE);
+#pragma unroll
+    for (int u = 0; u < W; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float x = w[u][i];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            const int j = u * K8_BLOCK + i * 8 + g;
+            if (t == 0 && j0 + j < s.len) wo[j] = old[u][i] + x;
+        }
 }
 
 }  // namespace qtts

@@ -35,57 +35,84 @@ __device__ __forceinline__ float2 rope_unit(int pos, double freq, float factor) 
     return make_float2(c * factor, s * factor);
 }
 
-// One warp per (row, run of heads).  A lane owns V consecutive dims of every
-// head, so it holds their cos / sin in registers for all heads of the run; the
-// partner values of a head go through shared memory, which serves every layout,
-// pair distance and rotated part alike.
-constexpr int ROPE_WARPS = 8;
-template <class T, int V>
+// One warp per (row, run of heads).  A lane owns the same 16 bytes of every head it
+// sees (L lanes a head, 32 / L heads at a time, 4 loads in flight), so it holds their
+// cos / sin in registers for the whole run.  Partners: in the lane's own word
+// (interleaved), 16 bytes of another lane through shared memory (half, rot / 2 a
+// multiple of the word), or single values of shared memory (any other rot).  Bound by
+// memory: every value is read and written once.
+constexpr int ROPE_WARPS = 8, ROPE_DEEP = 4;
+enum : int { ROPE_PAIR = 0, ROPE_WORD = 1, ROPE_VALUE = 2 };
+template <class T, int L, int MODE>
 __global__ void __launch_bounds__(ROPE_WARPS * 32) k_rope(RopeArgs a) {
-    constexpr int D = V * 32;
+    constexpr int V = 16 / sizeof(T), D = L * V, HPW = 32 / L;
+    struct alignas(16) Vec { T x[V]; };
     __shared__ float2 s_cs[ROPE_WARPS][D / 2];
-    __shared__ __align__(16) T s_x[ROPE_WARPS][D];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ Vec s_x[MODE == ROPE_PAIR ? 1 : ROPE_WARPS][ROPE_DEEP][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / L, d0 = lane % L * V;
     const int64_t unit = (int64_t) blockIdx.x * ROPE_WARPS + warp;
     const int64_t row = unit / a.chunks;
+    pdl_trigger();
+    pdl_wait();
     if (row >= a.rows) return;
-    const int h0 = (int)(unit % a.chunks) * a.heads_per_warp;
-    const int h1 = min(a.q_heads + a.k_heads, h0 + a.heads_per_warp);
-    const int half = a.rot >> 1, pos = a.pos[row];
+    const int h0 = (int)(unit % a.chunks) * a.heads_per_warp, heads = a.q_heads + a.k_heads, h1 = min(heads, h0 + a.heads_per_warp);
+    const int half = a.rot >> 1;
+    auto at = [&](int h, bool out) {
+        const bool is_q = h < a.q_heads;
+        const int64_t r = is_q ? (out ? a.qo_row : a.qs_row) : (out ? a.ko_row : a.ks_row), hs = is_q ? (out ? a.qo_head : a.qs_head) : (out ? a.ko_head : a.ks_head);
+        const void * p = is_q ? (out ? a.q_out : a.q) : (out ? a.k_out : a.k);
+        return const_cast<T *>(static_cast<const T *>(p)) + row * r + (is_q ? h : h - a.q_heads) * hs + d0;
+    };
+    Vec x[ROPE_DEEP];
+    auto load = [&](int hb) {
+#pragma unroll
+        for (int i = 0; i < ROPE_DEEP; ++i) {
+            const int h = hb + i * HPW + sub;
+            if (h < h1) x[i] = *reinterpret_cast<const Vec *>(at(h, false));
+        }
+    };
+    load(h0);
+    const int pos = a.pos[row];
     for (int i = lane; i < half; i += 32) s_cs[warp][i] = rope_unit(pos, a.freq[i], a.factor);
     __syncwarp();
     float c[V], s[V];
     int partner[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const int d = lane * V + e;
+        const int d = d0 + e;
         c[e] = 1.0f; s[e] = 0.0f; partner[e] = d;
         if (d < a.rot) {
-            const int i = a.interleaved ? d >> 1 : (d < half ? d : d - half);
-            const bool first = a.interleaved ? !(d & 1) : d < half;
+            const int i = MODE == ROPE_PAIR ? d >> 1 : (d < half ? d : d - half);
+            const bool first = MODE == ROPE_PAIR ? !(d & 1) : d < half;
             const float2 u = s_cs[warp][i];
             c[e] = u.x;
             s[e] = first ? -u.y : u.y;
-            partner[e] = a.interleaved ? d ^ 1 : (first ? d + half : d - half);
+            partner[e] = first ? d + half : d - half;
         }
     }
-    struct alignas(sizeof(T) * V) Vec { T x[V]; };
-    for (int h = h0; h < h1; ++h) {
-        const bool is_q = h < a.q_heads;
-        const int hh = is_q ? h : h - a.q_heads;
-        const T * src = static_cast<const T *>(is_q ? a.q : a.k) + row * (is_q ? a.qs_row : a.ks_row) + hh * (is_q ? a.qs_head : a.ks_head);
-        T * dst = static_cast<T *>(is_q ? a.q_out : a.k_out) + row * (is_q ? a.qo_row : a.ko_row) + hh * (is_q ? a.qo_head : a.ko_head);
-        const Vec x = *reinterpret_cast<const Vec *>(src + lane * V);
-        *reinterpret_cast<Vec *>(&s_x[warp][lane * V]) = x;
-        __syncwarp();
-        Vec y;
+    for (int hb = h0; hb < h1; hb += ROPE_DEEP * HPW) {
+        if (hb != h0) load(hb);
+        if (MODE != ROPE_PAIR) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float o = (float) s_x[warp][partner[e]];
-            y.x[e] = lane * V + e < a.rot ? T(__fmaf_rn((float) x.x[e], c[e], __fmul_rn(o, s[e]))) : x.x[e];
+            for (int i = 0; i < ROPE_DEEP; ++i) s_x[warp][i][lane] = x[i];
+            __syncwarp();
         }
-        *reinterpret_cast<Vec *>(dst + lane * V) = y;
-        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < ROPE_DEEP; ++i) {
+            const int h = hb + i * HPW + sub;
+            Vec o, y;
+            if (MODE == ROPE_WORD) o = s_x[warp][i][sub * L + partner[0] / V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                float p;
+                if (MODE == ROPE_PAIR) p = (float) x[i].x[e ^ 1];
+                else if (MODE == ROPE_WORD) p = (float) o.x[e];
+                else p = (float) reinterpret_cast<const T *>(&s_x[warp][i][sub * L])[partner[e]];
+                y.x[e] = d0 + e < a.rot ? T(__fmaf_rn((float) x[i].x[e], c[e], __fmul_rn(p, s[e]))) : x[i].x[e];
+            }
+            if (h < h1) *reinterpret_cast<Vec *>(at(h, true)) = y;
+        }
+        if (MODE != ROPE_PAIR) __syncwarp();
     }
 }
 
@@ -94,6 +121,8 @@ template <class T>
 __global__ void __launch_bounds__(256) k_rope_any(RopeArgs a) {
     const int half = a.rot >> 1, units = a.dim - half, heads = a.q_heads + a.k_heads;
     const int64_t total = (int64_t) a.rows * heads * units;
+    pdl_trigger();
+    pdl_wait();
     for (int64_t t = (int64_t) blockIdx.x * blockDim.x + threadIdx.x; t < total; t += (int64_t) gridDim.x * blockDim.x) {
         const int u = (int)(t % units), h = (int)(t / units % heads);
         const int64_t row = t / units / heads;

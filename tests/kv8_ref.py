@@ -26,13 +26,14 @@ def rope(x, pos, freq, layout, factor):
 
 
 def quantise(rows, code):
-    """Blocks [..., 16, D] -> (codes, scales [...]), the definition's float32 steps."""
+    """Blocks [..., 16, D] -> (codes, scales [...]): the largest magnitude over top, rounded
+    to float32, and the exact quotients x top / amax rounded to codes."""
     x = rows.float()
     most = x.abs().amax((-1, -2))
     fine = torch.isfinite(most)
     top = TOP[code]
     scale = torch.where(fine, most / top, torch.full_like(most, math.nan))
-    r = (x / scale[..., None, None]).clamp(-top, top)
+    r = (x.double() * top / most.double()[..., None, None]).float()
     r = torch.where((fine & (most > 0))[..., None, None], r, torch.zeros_like(r))
     return (r.round() if code == "int8" else r).to(CODE[code]), scale
 

@@ -219,6 +219,27 @@ def test_append_of_values_at_the_edges(kv8):
         assert bool(torch.isnan(k[0][48:]).all()) and bool(torch.isfinite(k[0][:48]).all()) and bool(torch.isnan(v[0][:48]).all())
 
 
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_append_rounds_every_quotient_correctly(kv8, code, dtype):
+    """Every mantissa of a block's largest magnitude against every value of the eleven binades below it (F16; all of BF16's
+    mantissas twice over): ties are exact quotients, so one wrong bit of a quotient shows."""
+    bits = 10 if dtype is F16 else 7
+    m = torch.arange(2 ** bits, dtype=torch.float64) / 2 ** bits + 1
+    below = torch.cat([m * 2.0 ** -e for e in range(11)])                       # 11 * 2^bits values up to 2
+    per = 11 if dtype is F16 else 2
+    x = torch.zeros(2 ** bits, per, 1024, dtype=torch.float64)
+    v = below.repeat(2)[: per * 1023].reshape(per, 1023)
+    x[:, :, 1:] = torch.minimum(v[None], m[:, None, None])
+    x[:, :, 0] = m[:, None]
+    x[:, :, 2::3] *= -1
+    x = x.reshape(-1, 1, 64).to(dtype)
+    n = x.shape[0]
+    a = Both(kv8, 1, 1, 64, code, dtype, cols=-(-n // 64))
+    a.append([n], x, x.flip(0).contiguous())
+    a.same()
+
+
 @pytest.mark.parametrize("pad", [0, 1, 8])
 def test_append_of_strided_rows(kv8, pad):
     a = Both(kv8, 3, 2, 128, "int8", BF16, cols=2)
