@@ -105,8 +105,8 @@ template <class T> int32_t rope_launch(const RopeArgs & a, cudaStream_t st) {
         b.chunks = (heads + b.heads_per_warp - 1) / b.heads_per_warp;
         unsigned g;
         if (!grid_of((int64_t) a.rows * b.chunks, ROPE_WARPS, &g)) return refuse("qtts_op_rope", "too many rows");
-        if (a.interleaved) e = rope_go<T, ROPE_PAIR>(b, g, lanes, st);
-        else if (a.rot / 2 % V == 0) e = rope_go<T, ROPE_WORD>(b, g, lanes, st);
+        if (a.interleaved && a.rot % V == 0) e = rope_go<T, ROPE_PAIR>(b, g, lanes, st);
+        else if (!a.interleaved && a.rot / 2 % V == 0) e = rope_go<T, ROPE_WORD>(b, g, lanes, st);
         else e = rope_go<T, ROPE_VALUE>(b, g, lanes, st);
     }
     return result("qtts_op_rope", e);

@@ -35,20 +35,54 @@ __device__ __forceinline__ float2 rope_unit(int pos, double freq, float factor) 
     return make_float2(c * factor, s * factor);
 }
 
+// Two 16-bit values of a word as floats, and back (one rounding each).
+template <class T> __device__ __forceinline__ float2 rope_up(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+template <> __device__ __forceinline__ float2 rope_up<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+template <class T> __device__ __forceinline__ uint32_t rope_down(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t rope_down<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// 16 bytes as floats.
+template <class T> struct RopeWord {
+    static constexpr int V = 16 / sizeof(T);
+    float x[V];
+    __device__ __forceinline__ explicit RopeWord(const uint4 & u) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w[i]);
+            else { const float2 f = rope_up<T>(w[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+        }
+    }
+    __device__ __forceinline__ uint4 pack() const {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(x[i]);
+            else w[i] = rope_down<T>(x[2 * i], x[2 * i + 1]);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
 // One warp per (row, run of heads).  A lane owns the same 16 bytes of every head it
-// sees (L lanes a head, 32 / L heads at a time, 4 loads in flight), so it holds their
-// cos / sin in registers for the whole run.  Partners: in the lane's own word
-// (interleaved), 16 bytes of another lane through shared memory (half, rot / 2 a
-// multiple of the word), or single values of shared memory (any other rot).  Bound by
-// memory: every value is read and written once.
-constexpr int ROPE_WARPS = 8, ROPE_DEEP = 4;
+// sees (L lanes a head, 32 / L heads at a time), so it holds their cos / sin in
+// registers for the whole run; the next heads' loads are in flight while these are
+// turned.  Partners: in the lane's own word (interleaved), 16 bytes of another lane
+// through shared memory (half), or, where the rotated part does not end or split at a
+// word, single values of shared memory.  Bound by memory: every value is read and
+// written once.
+constexpr int ROPE_WARPS = 8, ROPE_DEEP = 2;
 enum : int { ROPE_PAIR = 0, ROPE_WORD = 1, ROPE_VALUE = 2 };
 template <class T, int L, int MODE>
 __global__ void __launch_bounds__(ROPE_WARPS * 32) k_rope(RopeArgs a) {
     constexpr int V = 16 / sizeof(T), D = L * V, HPW = 32 / L;
-    struct alignas(16) Vec { T x[V]; };
     __shared__ float2 s_cs[ROPE_WARPS][D / 2];
-    __shared__ Vec s_x[MODE == ROPE_PAIR ? 1 : ROPE_WARPS][ROPE_DEEP][32];
+    __shared__ uint4 s_x[MODE == ROPE_PAIR ? 1 : ROPE_WARPS][ROPE_DEEP][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / L, d0 = lane % L * V;
     const int64_t unit = (int64_t) blockIdx.x * ROPE_WARPS + warp;
     const int64_t row = unit / a.chunks;
@@ -57,62 +91,67 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) k_rope(RopeArgs a) {
     if (row >= a.rows) return;
     const int h0 = (int)(unit % a.chunks) * a.heads_per_warp, heads = a.q_heads + a.k_heads, h1 = min(heads, h0 + a.heads_per_warp);
     const int half = a.rot >> 1;
-    auto at = [&](int h, bool out) {
-        const bool is_q = h < a.q_heads;
-        const int64_t r = is_q ? (out ? a.qo_row : a.qs_row) : (out ? a.ko_row : a.ks_row), hs = is_q ? (out ? a.qo_head : a.qs_head) : (out ? a.ko_head : a.ks_head);
-        const void * p = is_q ? (out ? a.q_out : a.q) : (out ? a.k_out : a.k);
-        return const_cast<T *>(static_cast<const T *>(p)) + row * r + (is_q ? h : h - a.q_heads) * hs + d0;
-    };
-    Vec x[ROPE_DEEP];
+    // key heads follow the query heads: head h of k at k + (h - q_heads) * stride
+    const T * qi = static_cast<const T *>(a.q) + row * a.qs_row + d0, * ki = static_cast<const T *>(a.k) + row * a.ks_row - a.q_heads * a.ks_head + d0;
+    T * qo = static_cast<T *>(a.q_out) + row * a.qo_row + d0, * ko = static_cast<T *>(a.k_out) + row * a.ko_row - a.q_heads * a.ko_head + d0;
+    uint4 x[ROPE_DEEP];
     auto load = [&](int hb) {
 #pragma unroll
         for (int i = 0; i < ROPE_DEEP; ++i) {
             const int h = hb + i * HPW + sub;
-            if (h < h1) x[i] = *reinterpret_cast<const Vec *>(at(h, false));
+            if (h < h1) x[i] = *reinterpret_cast<const uint4 *>(h < a.q_heads ? qi + h * a.qs_head : ki + h * a.ks_head);
         }
     };
+#pragma unroll
+    for (int i = 0; i < ROPE_DEEP; ++i) x[i] = make_uint4(0, 0, 0, 0);
     load(h0);
     const int pos = a.pos[row];
     for (int i = lane; i < half; i += 32) s_cs[warp][i] = rope_unit(pos, a.freq[i], a.factor);
     __syncwarp();
     float c[V], s[V];
     int partner[V];
+    bool turned[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int d = d0 + e;
+        turned[e] = MODE == ROPE_VALUE ? d < a.rot : d0 < a.rot;
         c[e] = 1.0f; s[e] = 0.0f; partner[e] = d;
         if (d < a.rot) {
-            const int i = MODE == ROPE_PAIR ? d >> 1 : (d < half ? d : d - half);
-            const bool first = MODE == ROPE_PAIR ? !(d & 1) : d < half;
+            const int i = a.interleaved ? d >> 1 : (d < half ? d : d - half);
+            const bool first = a.interleaved ? !(d & 1) : d < half;
             const float2 u = s_cs[warp][i];
             c[e] = u.x;
             s[e] = first ? -u.y : u.y;
-            partner[e] = first ? d + half : d - half;
+            partner[e] = a.interleaved ? d ^ 1 : (first ? d + half : d - half);
         }
     }
     for (int hb = h0; hb < h1; hb += ROPE_DEEP * HPW) {
-        if (hb != h0) load(hb);
-        if (MODE != ROPE_PAIR) {
+        uint4 now[ROPE_DEEP];
 #pragma unroll
-            for (int i = 0; i < ROPE_DEEP; ++i) s_x[warp][i][lane] = x[i];
+        for (int i = 0; i < ROPE_DEEP; ++i) now[i] = x[i];
+        if (hb + ROPE_DEEP * HPW < h1) load(hb + ROPE_DEEP * HPW);
+        if (MODE != ROPE_PAIR) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < ROPE_DEEP; ++i) s_x[warp][i][lane] = now[i];
             __syncwarp();
         }
 #pragma unroll
         for (int i = 0; i < ROPE_DEEP; ++i) {
             const int h = hb + i * HPW + sub;
-            Vec o, y;
-            if (MODE == ROPE_WORD) o = s_x[warp][i][sub * L + partner[0] / V];
+            uint4 y = now[i];
+            if (turned[0]) {
+                RopeWord<T> v(now[i]), o(MODE == ROPE_WORD ? s_x[warp][i][sub * L + partner[0] / V] : now[i]), r(now[i]);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                float p;
-                if (MODE == ROPE_PAIR) p = (float) x[i].x[e ^ 1];
-                else if (MODE == ROPE_WORD) p = (float) o.x[e];
-                else p = (float) reinterpret_cast<const T *>(&s_x[warp][i][sub * L])[partner[e]];
-                y.x[e] = d0 + e < a.rot ? T(__fmaf_rn((float) x[i].x[e], c[e], __fmul_rn(p, s[e]))) : x[i].x[e];
+                for (int e = 0; e < V; ++e) {
+                    const float p = MODE == ROPE_PAIR ? v.x[e ^ 1]
+                                  : MODE == ROPE_WORD ? o.x[e] : (float) reinterpret_cast<const T *>(&s_x[warp][i][sub * L])[partner[e]];
+                    if (MODE != ROPE_VALUE || turned[e]) r.x[e] = __fmaf_rn(v.x[e], c[e], __fmul_rn(p, s[e]));
+                }
+                y = r.pack();                         // values that do not turn come back as they were: the conversions are exact
             }
-            if (h < h1) *reinterpret_cast<Vec *>(at(h, true)) = y;
+            if (h < h1) *reinterpret_cast<uint4 *>(h < a.q_heads ? qo + h * a.qo_head : ko + h * a.ko_head) = y;
         }
-        if (MODE != ROPE_PAIR) __syncwarp();
     }
 }
 
