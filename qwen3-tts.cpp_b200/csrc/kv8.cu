@@ -8,6 +8,7 @@
 
 #include "kv8.cuh"
 #include "kv8_attend.cuh"
+#include "kv8_tile.cuh"
 #include "rope.cuh"
 
 namespace qtts {
@@ -130,23 +131,27 @@ template <class F> void by_cache(const qtts_kv8 & c, F f) {
     else by_code(__nv_bfloat16{});
 }
 
-// How an attention call runs.  Rows of a (sequence, kv head) come in tiles of 8 nt;
-// one CTA takes a tile's whole range, or, with few tiles over a long cache, the
-// ranges are split evenly over the GPU.
-struct K8Plan { int nt, tiles, split, ctas, part_rows; int64_t line_bytes, part_bytes; unsigned grid; };   // workspace: line, parts, lse
+// How an attention call runs.  Up to 64 rows of a (sequence, kv head) come in tiles of
+// 8 nt; one CTA takes a tile's whole range, or, where that is more than 8 pages, the
+// ranges are split evenly over the GPU.  More rows come in tiles of 256 on tcgen05.
+enum : int { PLAN_WHOLE, PLAN_SPLIT, PLAN_TILE };
+struct K8Plan { int kind, nt, tiles, ctas, part_rows; int64_t line_bytes, part_bytes; unsigned grid; };   // workspace: line, parts, lse
 constexpr int SMS = 148, NW = 4;
 bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     const int64_t R = (int64_t) p.max_q * (p.n_heads / c.n_kv_heads);
+    const bool tile = R > 64 && c.head_dim <= 128;
     o->nt = R <= 8 ? 1 : (R <= 16 || c.head_dim == 256 ? 2 : 4);
-    const int64_t tiles = (R + 8 * o->nt - 1) / (8 * o->nt), items = tiles * c.n_kv_heads * c.n_seqs;
+    const int per = tile ? KT_ROWS : 8 * o->nt;
+    const int64_t tiles = (R + per - 1) / per, items = tiles * c.n_kv_heads * c.n_seqs;
     if (items > 0x7fffffff) return false;
+    const bool split = !tile && c.max_pages > 8 && R <= 64 && c.n_seqs <= K8_MAX_SPLIT_SEQS && items * c.max_pages < 0x40000000;
+    o->kind = tile ? PLAN_TILE : (split ? PLAN_SPLIT : PLAN_WHOLE);
     o->tiles = (int) tiles;
-    o->split = c.max_pages > 8 && R <= 64 && c.n_seqs <= K8_MAX_SPLIT_SEQS && items * c.max_pages < 0x40000000;
     o->ctas = SMS * k8_ctas_per_sm(c.head_dim, o->nt);
     o->part_rows = (int)(R < 8 * o->nt ? R : 8 * o->nt);
-    o->line_bytes = o->split ? ((int64_t) c.n_seqs + 4) / 4 * 16 : 0;
-    o->part_bytes = o->split ? (int64_t) o->ctas * 2 * o->part_rows * (c.head_dim + 4) * 4 : 0;
-    o->grid = (unsigned)(o->split ? o->ctas : items);
+    o->line_bytes = split ? ((int64_t) c.n_seqs + 4) / 4 * 16 : 0;
+    o->part_bytes = split ? (int64_t) o->ctas * 2 * o->part_rows * (c.head_dim + 4) * 4 : 0;
+    o->grid = (unsigned)(split ? o->ctas : items);
     return true;
 }
 // The shared memory limit of a kernel, raised once per device.
@@ -182,7 +187,7 @@ cudaError_t attend_launch(const K8AttendArgs & a, const K8Plan & p, cudaStream_t
     constexpr int rows = K8_U<D, NT> * K8_BLOCK;
     if (!make_map(&maps.k, a.c.k, a.c, rows) || !make_map(&maps.v, a.c.v, a.c, rows)) return cudaErrorNotSupported;
     constexpr int base = k8_smem_bytes<D, NT, NW>();
-    if (!p.split) {
+    if (p.kind == PLAN_WHOLE) {
         constexpr auto f = k_kv8_attend_whole<T, E4M3, D, NT, NW>;
         const cudaError_t e = allow_smem<f>(base, a.c.device);
         if (e != cudaSuccess) return e;
@@ -195,6 +200,15 @@ cudaError_t attend_launch(const K8AttendArgs & a, const K8Plan & p, cudaStream_t
     if ((e = pdl_go(f, p.grid, NW * 32, smem, st, a, maps)) != cudaSuccess) return e;
     return pdl_go(k_kv8_join<T, D, NT>, (unsigned)((int64_t) a.c.n_seqs * a.c.n_kv_heads * a.max_q * (a.n_heads / a.c.n_kv_heads)), K8_JOIN_WARPS * 32,
                   0, st, a);
+}
+
+template <class T, bool E4M3, int D>
+cudaError_t tile_launch(const K8AttendArgs & a, const K8Plan & p, cudaStream_t st) {
+    K8Maps maps;
+    if (!make_map(&maps.k, a.c.k, a.c, K8_PAGE) || !make_map(&maps.v, a.c.v, a.c, K8_PAGE)) return cudaErrorNotSupported;
+    constexpr auto f = k_kv8_attend_tile<T, E4M3, D>;
+    const cudaError_t e = allow_smem<f>(KtSmem<D>::total, a.c.device);
+    return e != cudaSuccess ? e : pdl_go(f, p.grid, KT_THREADS, KtSmem<D>::total, st, a, maps);
 }
 
 }  // namespace
@@ -378,7 +392,9 @@ int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * p, void *
         constexpr bool E = decltype(e)::value;
         constexpr int D = decltype(d)::value;
         if (p->n_rows > 0 && p->max_q > 0) {
-            if (plan.nt == 1) err = attend_launch<T, E, D, 1>(a, plan, st);
+            if (plan.kind == PLAN_TILE) {
+                if constexpr (D < 256) err = tile_launch<T, E, D>(a, plan, st);
+            } else if (plan.nt == 1) err = attend_launch<T, E, D, 1>(a, plan, st);
             else if (plan.nt == 2) err = attend_launch<T, E, D, 2>(a, plan, st);
             else if constexpr (D < 256) err = attend_launch<T, E, D, 4>(a, plan, st);
         }
