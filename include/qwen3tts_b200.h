@@ -349,6 +349,7 @@ int32_t qtts_op_kv8_read(const qtts_kv8 * c, const int32_t * table, const int32_
 /* Attention of q [n_rows][n_heads][head_dim] (row_type) over the cache: sequence b
  * brings rows cu[b] .. cu[b+1]-1 (cu NULL: one each), the last of them at position
  * lens[b]-1; row at position p sees keys j <= p and, with window > 0, j > p - window.
+ * scale (on the products of q and k) is finite and not negative.
  * A row that sees nothing gives zeros (lse -inf); rows of `out` that belong to no
  * sequence stay as they were.  lse [n_rows][n_heads] F32 or NULL.  weight_in /
  * weight_out [n_seqs][n_kv_heads] at weight_stride (both NULL: none; they may be

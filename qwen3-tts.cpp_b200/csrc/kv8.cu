@@ -363,6 +363,7 @@ int32_t qtts_op_kv8_attend(const qtts_kv8 * c, const qtts_kv8_attend * p, void *
     if (p->n_heads < 1 || p->n_heads % c->n_kv_heads) return refuse(who, "n_heads is a multiple of n_kv_heads");
     if (p->n_rows < 0 || p->max_q < 0 || p->window < 0) return refuse(who, "n_rows, max_q or window");
     if (!p->cu && p->n_rows != c->n_seqs) return refuse(who, "without cu there is one row for each sequence");
+    if (!(p->scale >= 0.0f) || std::isinf(p->scale)) return refuse(who, "scale is finite and not negative");
     if ((p->weight_in == nullptr) != (p->weight_out == nullptr)) return refuse(who, "weight_in and weight_out go together");
     if (p->weight_out && p->weight_stride < (int64_t) c->max_pages * K8_PAGE) return refuse(who, "weight_stride is at least 64 max_pages");
     if (c->n_seqs == 0) return 1;

@@ -43,6 +43,19 @@ __device__ __forceinline__ void kt_sts(uint32_t p, uint32_t x, uint32_t y, uint3
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// Two F32 operations in one instruction.
+__device__ __forceinline__ float2 kt_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)), "l"(reinterpret_cast<const uint64_t &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 kt_add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(d)) : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
+    return d;
+}
+
 template <class T, bool E4M3, int D>
 __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs a, const __grid_constant__ K8Maps maps) {
     using M = KtSmem<D>;
@@ -172,25 +185,30 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
             const int beyond = none ? 0 : any_hi - (t0 + j) * K8_PAGE;      // keys from here on may hold anything
             const uint32_t raw = sb + M::raw_at + st * M::raw, out = sb + M::kv_at + kv * M::kv;
             constexpr int UNITS = 8 * (D / 64);                             // (key group, chunk group) pairs of a side
+            auto convert = [&](auto cut) {
 #pragma unroll
-            for (int side = 0; side < 2; ++side)
+                for (int side = 0; side < 2; ++side)
 #pragma unroll
-                for (int u0 = 0; u0 < UNITS / 4; ++u0) {
-                    const int u = u0 * 4 + (warp - 8), kg = u % 8, chunk = u / 8 * 4 + c_lo, key = kg * 8 + key_lo;
-                    const int sw = D == 64 ? chunk ^ (key >> 1 & 3) : chunk ^ key_lo;
-                    uint4 x = k8_lds16(raw + side * M::raw_side + key * D + sw * 16);
-                    if (key >= beyond) x = make_uint4(0, 0, 0, 0);
-                    uint32_t f[8];
-                    k8_f16x4<E4M3>(x.x, f[0], f[1]);
-                    k8_f16x4<E4M3>(x.y, f[2], f[3]);
-                    k8_f16x4<E4M3>(x.z, f[4], f[5]);
-                    k8_f16x4<E4M3>(x.w, f[6], f[7]);
-                    // K: [k tile of 64 dims][key group][8 dims][key], V: [key group][8 dims][key], 16 bytes each
-                    const uint32_t p = side == 0 ? out + (chunk >> 2) * 8192 + kg * 1024 + (chunk & 3) * 256 + key_lo * 16
-                                                 : out + M::f16_side + kg * (D * 16) + chunk * 256 + key_lo * 16;
-                    kt_sts(p, f[0], f[1], f[2], f[3]);
-                    kt_sts(p + 128, f[4], f[5], f[6], f[7]);
-                }
+                    for (int u0 = 0; u0 < UNITS / 4; ++u0) {
+                        // unit u0 * 4 + (warp - 8): key group u % 8, chunk group u / 8
+                        const int kg = (u0 & 1) * 4 + (warp - 8), c4 = u0 >> 1, chunk = c4 * 4 + c_lo, key = kg * 8 + key_lo;
+                        const int sw = D == 64 ? chunk ^ (key_lo >> 1) : chunk ^ key_lo;
+                        uint4 x = k8_lds16(raw + side * M::raw_side + key * D + sw * 16);
+                        if (decltype(cut)::value && key >= beyond) x = make_uint4(0, 0, 0, 0);
+                        uint32_t f[8];
+                        k8_f16x4<E4M3>(x.x, f[0], f[1]);
+                        k8_f16x4<E4M3>(x.y, f[2], f[3]);
+                        k8_f16x4<E4M3>(x.z, f[4], f[5]);
+                        k8_f16x4<E4M3>(x.w, f[6], f[7]);
+                        // K: [k tile of 64 dims][key group][8 dims][key], V: [key group][8 dims][key], 16 bytes each
+                        const uint32_t p = side == 0 ? out + c4 * 8192 + kg * 1024 + c_lo * 256 + key_lo * 16
+                                                     : out + M::f16_side + kg * (D * 16) + chunk * 256 + key_lo * 16;
+                        kt_sts(p, f[0], f[1], f[2], f[3]);
+                        kt_sts(p + 128, f[4], f[5], f[6], f[7]);
+                    }
+            };
+            if (beyond >= K8_PAGE) convert(std::false_type{});
+            else convert(std::true_type{});
             if (threadIdx.x - 256 < 9) scales(KT_RAW + kv)[threadIdx.x - 256] = scales(st)[threadIdx.x - 256];
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             kt_arrive(bar + KT_KV_FULL + kv);
@@ -247,25 +265,26 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
             if (!ok) break;
             tc_fence_after();
             float sv[K8_PAGE];
-#pragma unroll
-            for (int c = 0; c < K8_PAGE; c += 16) tc_ld16_nowait(tm_s + (j & 1) * K8_PAGE + c, sv + c);
+            tc_ld_wait<K8_PAGE>(tm_s + (j & 1) * K8_PAGE, sv);
             const float * sc = scales(KT_RAW + (j & 1));
             const int kb = (t0 + j) * K8_PAGE;
             const bool none = reinterpret_cast<const int *>(sc)[8] != 0;
             const bool whole = !none && kb >= all_lo && kb + K8_PAGE <= all_hi;
             float ks[4], vs[4], mx = -INFINITY;
+            bool plain = whole;                                             // every row sees every key, and no scale of V is NaN
 #pragma unroll
-            for (int u = 0; u < 4; ++u) { ks[u] = sc[u] * fac; vs[u] = sc[4 + u]; }
-            tc_wait_ld();
-            if (whole) {
+            for (int u = 0; u < 4; ++u) { ks[u] = sc[u] * fac; vs[u] = sc[4 + u]; plain = plain && vs[u] == vs[u]; }
+            if (!whole) {
 #pragma unroll
-                for (int i = 0; i < K8_PAGE; ++i) { sv[i] *= ks[i >> 4]; mx = fmaxf(mx, sv[i]); }
-            } else {
+                for (int i = 0; i < K8_PAGE; ++i)
+                    if (none || kb + i < lo || kb + i >= hi) sv[i] = -INFINITY;
+            }
 #pragma unroll
-                for (int i = 0; i < K8_PAGE; ++i) {
-                    sv[i] = none || kb + i < lo || kb + i >= hi ? -INFINITY : sv[i] * ks[i >> 4];
-                    mx = fmaxf(mx, sv[i]);
-                }
+            for (int u = 0; u < 4; ++u) {                                   // scales are not negative: the largest score of 16 keys is the largest product's
+                float x = sv[16 * u];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) x = fmaxf(x, sv[16 * u + i]);
+                mx = fmaxf(mx, x == -INFINITY ? x : x * ks[u]);
             }
             const float top = none ? 0.0f : fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
             const bool up = __any_sync(0xffffffffu, mx > m + K8_SLACK || top > unit * K8_UNIT_SLACK);
@@ -281,9 +300,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
 #pragma unroll
                     for (int c = 0; c < D; c += 32) {
                         float o[32];
-                        tc_ld16_nowait(tm_o + c, o);
-                        tc_ld16_nowait(tm_o + c + 16, o + 16);
-                        tc_wait_ld();
+                        tc_ld_wait<32>(tm_o + c, o);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] *= f;
                         tc_st16(tm_o + c, o);
@@ -293,18 +310,44 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
                 }
             }
             const float inv = __fdividef(1.0f, unit), ref = m - K8_LIFT;
+            if (plain) {
+                // 2^(s - ref) times a block's V scale over `unit` as one exponential; the sum takes the factor back.  A
+                // block of zeros (scale 0) keeps the factor 1, and below 2^-60 nothing is left of it in F16 either way.
 #pragma unroll
-            for (int c = 0; c < K8_PAGE / 8; ++c) {
-                const float rv = vs[c >> 1] * inv;
-                float e[8];
+                for (int u = 0; u < 4; ++u) {
+                    const float rv = vs[u] == 0.0f ? 1.0f : fmaxf(vs[u] * inv, 8.6736173798840355e-19f);
+                    const float off = __log2f(rv) - ref;
+                    const float2 k2 = make_float2(ks[u], ks[u]), o2 = make_float2(off, off);
+                    float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = k8_exp2(sv[c * 8 + i] - ref);
-                    const bool hidden = !whole && sv[c * 8 + i] == -INFINITY;
-                    e[i] = hidden ? 0.0f : x * rv;
-                    l += hidden ? 0.0f : x;
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t pk[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float2 x = kt_fma2(make_float2(sv[16 * u + 8 * c + 2 * i], sv[16 * u + 8 * c + 2 * i + 1]), k2, o2);
+                            x.x = k8_exp2(x.x);
+                            x.y = k8_exp2(x.y);
+                            sum = kt_add2(sum, x);
+                            pk[i] = k8_pack(x.x, x.y);
+                        }
+                        kt_sts(pw + (2 * u + c) * 128, pk[0], pk[1], pk[2], pk[3]);
+                    }
+                    l += __fdividef(sum.x + sum.y, rv);
                 }
-                kt_sts(pw + c * 128, k8_pack(e[0], e[1]), k8_pack(e[2], e[3]), k8_pack(e[4], e[5]), k8_pack(e[6], e[7]));
+            } else {
+#pragma unroll
+                for (int c = 0; c < K8_PAGE / 8; ++c) {
+                    const float rv = vs[c >> 1] * inv;
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float x = k8_exp2(fmaf(sv[c * 8 + i], ks[c >> 1], -ref));
+                        const bool hidden = sv[c * 8 + i] == -INFINITY;
+                        e[i] = hidden ? 0.0f : x * rv;
+                        l += hidden ? 0.0f : x;
+                    }
+                    kt_sts(pw + c * 128, k8_pack(e[0], e[1]), k8_pack(e[2], e[3]), k8_pack(e[4], e[5]), k8_pack(e[6], e[7]));
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_before();
@@ -320,10 +363,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
 #pragma unroll
             for (int c = 0; c < D; c += 16) {
                 float o[16];
-                if (mine > 0) {                                             // the same for the whole warp
-                    tc_ld16_nowait(tm_o + c, o);
-                    tc_wait_ld();
-                }
+                if (mine > 0) tc_ld_wait<16>(tm_o + c, o);                  // the same for the whole warp
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[i] = mine > 0 && l != 0.0f ? o[i] * f : 0.0f;
                 if (real) {

@@ -67,7 +67,7 @@ def test_refusals_of_attend(kv8):
         return L.qtts_op_kv8_attend(c, C.byref(a), None)
 
     for kw in [dict(table=None), dict(lens=None), dict(q=None), dict(out=None), dict(q=4097), dict(n_heads=3), dict(n_heads=0), dict(n_rows=2),
-               dict(n_rows=-1), dict(max_q=-1), dict(window=-1), dict(weight_in=4096), dict(weight_out=4096),
+               dict(n_rows=-1), dict(max_q=-1), dict(window=-1), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(weight_in=4096), dict(weight_out=4096),
                dict(weight_in=4096, weight_out=4096, weight_stride=255), dict(weight_in=4096, weight_out=4096, weight_stride=256)]:
         assert call(**kw) == 0, kw
     assert L.qtts_op_kv8_attend(c, None, None) == 0
