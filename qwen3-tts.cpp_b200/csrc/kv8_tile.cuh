@@ -141,14 +141,18 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
         if (lane == 0 && n > 0) {
             const uint32_t id_s = tc_idesc_f16(K8_PAGE, false), id_o = tc_idesc_f16(D, true);
             bool ok = mbar_wait(bar + KT_Q, 0);
+            // descriptors: low words stepped in units of 16 bytes
+            const uint64_t dq = tc_desc(sb + M::q_at, 128, 1024), dk = tc_desc(sb + M::kv_at, 128, 1024), dp = tc_desc(sb + M::p_at, 128, 1024),
+                           dv = tc_desc(sb + M::kv_at + M::f16_side, D * 16, 128);
+            const uint32_t k_hi = (uint32_t)(dk >> 32), v_hi = (uint32_t)(dv >> 32);   // (those of q and p are k's)
             auto scores = [&](int w, int j) {
                 ok = ok && mbar_wait(bar + KT_KV_FULL + (j & 1), (j >> 1) & 1);
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t q = sb + M::q_at + w * M::q, k = sb + M::kv_at + (j & 1) * M::kv, d = tmem + 2 * D + (w * 2 + (j & 1)) * K8_PAGE;
+                const uint32_t q = (uint32_t) dq + w * (M::q >> 4), k = (uint32_t) dk + (j & 1) * (M::kv >> 4), d = tmem + 2 * D + (w * 2 + (j & 1)) * K8_PAGE;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
-                    tc_mma(d, tc_desc(q + (i >> 2) * 16384 + (i & 3) * 256, 128, 1024), tc_desc(k + (i >> 2) * 8192 + (i & 3) * 256, 128, 1024), id_s, i > 0);
+                    tc_mma_lo(d, q + (i >> 2) * 1024 + (i & 3) * 16, k_hi, k + (i >> 2) * 512 + (i & 3) * 16, k_hi, id_s, i > 0);
                 tc_commit(bar + KT_S + w * 2 + (j & 1));
             };
             for (int w = 0; w < 2; ++w)
@@ -161,10 +165,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
                     ok = mbar_wait(bar + KT_P + w, j & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t p = sb + M::p_at + w * M::p, v = sb + M::kv_at + (j & 1) * M::kv + M::f16_side;
+                    const uint32_t p = (uint32_t) dp + w * (M::p >> 4), v = (uint32_t) dv + (j & 1) * (M::kv >> 4);
 #pragma unroll
-                    for (int i = 0; i < K8_PAGE / 16; ++i)
-                        tc_mma(tmem + w * D, tc_desc(p + i * 256, 128, 1024), tc_desc(v + i * 2 * D * 16, D * 16, 128), id_o, j > 0 || i > 0);
+                    for (int i = 0; i < K8_PAGE / 16; ++i) tc_mma_lo(tmem + w * D, p + i * 16, k_hi, v + i * 2 * D, v_hi, id_o, j > 0 || i > 0);
                     tc_commit(bar + KT_PV + w);
                 }
                 tc_commit(bar + KT_KV_EMPTY + (j & 1));

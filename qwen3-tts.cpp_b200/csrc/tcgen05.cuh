@@ -49,6 +49,16 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, float v[16]) {
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// MMA with the operands' descriptors as low words (address, lbo) that the caller steps in
+// units of 16 bytes, and common high words (sbo): a few instructions an MMA for the one
+// thread that issues them.
+__device__ __forceinline__ void tc_mma_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}\n"
+        ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc) : "memory");
+}
+
 // N columns of a lane's row, waited for in the same statement: the load writes its
 // registers some time after it was issued, and nothing else may be put into them (or
 // read from them, as a spill would) before the wait.
