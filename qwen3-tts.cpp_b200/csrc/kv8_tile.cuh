@@ -31,9 +31,12 @@ template <int D> struct KtSmem {
     static constexpr int f16_side = K8_PAGE * D * 2, kv = 2 * f16_side;              // a converted stage
     static constexpr int q = 128 * D * 2, p = 128 * K8_PAGE * 2;                     // per row tile
     static constexpr int raw_at = 0, kv_at = raw_at + KT_RAW * raw, q_at = kv_at + 2 * kv, p_at = q_at + 2 * q, scale_at = p_at + 2 * p;
-    static constexpr int bar_at = scale_at + (KT_RAW + 2) * 48, bytes = bar_at + 32 * 8 + 16, total = bytes + 1024;
+    static constexpr int bar_at = scale_at + (KT_RAW + 4) * 48, bytes = bar_at + 32 * 8 + 16, total = bytes + 1024;
 };
-enum : int { KT_RAW_FULL = 0, KT_RAW_EMPTY = 3, KT_KV_FULL = 6, KT_KV_EMPTY = 8, KT_Q = 10, KT_S = 11, KT_P = 15, KT_PV = 17, KT_DONE = 19, KT_BARS = 20 };
+// Barriers: raw stages filled / read (3 each); converted K and V stages filled / used (2 each); scales published (4);
+// query rows written; scores ready (tile, buffer); weights written, their product done (per tile); all MMAs done.
+enum : int { KT_RAW_FULL = 0, KT_RAW_EMPTY = 3, KT_K_FULL = 6, KT_V_FULL = 8, KT_K_EMPTY = 10, KT_V_EMPTY = 12, KT_SC = 14, KT_Q = 18, KT_S = 19, KT_P = 23,
+             KT_PV = 25, KT_DONE = 27, KT_BARS = 28 };
 
 __device__ __forceinline__ bool kt_wait(uint64_t * bar, int phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1)); }
 __device__ __forceinline__ void kt_arrive(uint64_t * bar) {
@@ -73,7 +76,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
     uint64_t * bar = reinterpret_cast<uint64_t *>(base + M::bar_at);
     uint32_t * s_tmem = reinterpret_cast<uint32_t *>(base + M::bar_at + 32 * 8);
     volatile int * s_fail = reinterpret_cast<volatile int *>(s_tmem + 1);
-    // scales of a ring or converted stage: 4 of K, 4 of V, then whether the page is none
+    // scales of a ring stage (0 ..) or published (KT_RAW ..): 4 of K, 4 of V, then whether the page is none
     auto scales = [&](int stage) { return reinterpret_cast<float *>(base + M::scale_at + stage * 48); };
 
     // pages [t0, t0 + nt[w]) for each tile of 128 rows
@@ -92,7 +95,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
     if (threadIdx.x == 0) {
         for (int i = 0; i < KT_BARS; ++i) {
             int count = 1;
-            if ((i >= KT_RAW_EMPTY && i < KT_KV_FULL) || (i >= KT_KV_FULL && i < KT_KV_EMPTY) || (i >= KT_P && i < KT_PV)) count = 128;
+            if ((i >= KT_RAW_EMPTY && i < KT_K_EMPTY) || (i >= KT_P && i < KT_PV)) count = 128;
             if (i == KT_Q) count = 256;
             mbar_init(bar + i, count);
         }
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
                            dv = tc_desc(sb + M::kv_at + M::f16_side, D * 16, 128);
             const uint32_t k_hi = (uint32_t)(dk >> 32), v_hi = (uint32_t)(dv >> 32);   // (those of q and p are k's)
             auto scores = [&](int w, int j) {
-                ok = ok && mbar_wait(bar + KT_KV_FULL + (j & 1), (j >> 1) & 1);
+                ok = ok && mbar_wait(bar + KT_K_FULL + (j & 1), (j >> 1) & 1);
                 if (!ok) return;
                 tc_fence_after();
                 const uint32_t q = (uint32_t) dq + w * (M::q >> 4), k = (uint32_t) dk + (j & 1) * (M::kv >> 4), d = tmem + 2 * D + (w * 2 + (j & 1)) * K8_PAGE;
@@ -155,14 +158,17 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
                     tc_mma_lo(d, q + (i >> 2) * 1024 + (i & 3) * 16, k_hi, k + (i >> 2) * 512 + (i & 3) * 16, k_hi, id_s, i > 0);
                 tc_commit(bar + KT_S + w * 2 + (j & 1));
             };
-            for (int w = 0; w < 2; ++w)
-                if (nt[w] > 0) scores(w, 0);
-            for (int j = 0; j < n && ok; ++j) {
+            auto both = [&](int j) {
                 for (int w = 0; w < 2; ++w)
-                    if (j + 1 < nt[w]) scores(w, j + 1);
+                    if (j < nt[w]) scores(w, j);
+                tc_commit(bar + KT_K_EMPTY + (j & 1));
+            };
+            both(0);
+            for (int j = 0; j < n && ok; ++j) {
+                if (j + 1 < n) both(j + 1);
                 for (int w = 0; w < 2 && ok; ++w) {
                     if (j >= nt[w]) continue;
-                    ok = mbar_wait(bar + KT_P + w, j & 1);
+                    ok = mbar_wait(bar + KT_P + w, j & 1) && mbar_wait(bar + KT_V_FULL + (j & 1), (j >> 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t p = (uint32_t) dp + w * (M::p >> 4), v = (uint32_t) dv + (j & 1) * (M::kv >> 4);
@@ -170,7 +176,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
                     for (int i = 0; i < K8_PAGE / 16; ++i) tc_mma_lo(tmem + w * D, p + i * 16, k_hi, v + i * 2 * D, v_hi, id_o, j > 0 || i > 0);
                     tc_commit(bar + KT_PV + w);
                 }
-                tc_commit(bar + KT_KV_EMPTY + (j & 1));
+                tc_commit(bar + KT_V_EMPTY + (j & 1));
             }
             if (!ok) *s_fail = 1;
             tc_commit(bar + KT_DONE);
@@ -178,45 +184,62 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
         }
     } else if (warp >= 8) {
         // ---- codes to F16: a lane takes 16 dims of a key; eight lanes the eight keys of a core matrix row group
+        // K of the next page before V of this one: K's stage is free when the scores are done, V's a whole softmax later
         const int key_lo = lane & 7, c_lo = lane >> 3;
-        for (int j = 0; j < n; ++j) {
-            const int st = j % KT_RAW, kv = j & 1;
-            bool ok = kt_wait(bar + KT_RAW_FULL + st, j / KT_RAW);
-            if (ok && j >= 2) ok = kt_wait(bar + KT_KV_EMPTY + kv, j / 2 - 1);
-            if (!ok) { if (lane == 0) *s_fail = 1; break; }
+        auto convert = [&](int side, int j) {
+            const int st = j % KT_RAW;
             const bool none = reinterpret_cast<const int *>(scales(st))[8] != 0;
             const int beyond = none ? 0 : any_hi - (t0 + j) * K8_PAGE;      // keys from here on may hold anything
-            const uint32_t raw = sb + M::raw_at + st * M::raw, out = sb + M::kv_at + kv * M::kv;
+            const uint32_t raw = sb + M::raw_at + st * M::raw + side * M::raw_side, out = sb + M::kv_at + (j & 1) * M::kv + side * M::f16_side;
             constexpr int UNITS = 8 * (D / 64);                             // (key group, chunk group) pairs of a side
-            auto convert = [&](auto cut) {
+            uint4 x[UNITS / 4];
 #pragma unroll
-                for (int side = 0; side < 2; ++side)
+            for (int u0 = 0; u0 < UNITS / 4; ++u0) {
+                // unit u0 * 4 + (warp - 8): key group u % 8, chunk group u / 8
+                const int key = ((u0 & 1) * 4 + (warp - 8)) * 8 + key_lo, chunk = (u0 >> 1) * 4 + c_lo, sw = D == 64 ? chunk ^ (key_lo >> 1) : chunk ^ key_lo;
+                x[u0] = k8_lds16(raw + key * D + sw * 16);
+            }
+            if (beyond < K8_PAGE)
 #pragma unroll
-                    for (int u0 = 0; u0 < UNITS / 4; ++u0) {
-                        // unit u0 * 4 + (warp - 8): key group u % 8, chunk group u / 8
-                        const int kg = (u0 & 1) * 4 + (warp - 8), c4 = u0 >> 1, chunk = c4 * 4 + c_lo, key = kg * 8 + key_lo;
-                        const int sw = D == 64 ? chunk ^ (key_lo >> 1) : chunk ^ key_lo;
-                        uint4 x = k8_lds16(raw + side * M::raw_side + key * D + sw * 16);
-                        if (decltype(cut)::value && key >= beyond) x = make_uint4(0, 0, 0, 0);
-                        uint32_t f[8];
-                        k8_f16x4<E4M3>(x.x, f[0], f[1]);
-                        k8_f16x4<E4M3>(x.y, f[2], f[3]);
-                        k8_f16x4<E4M3>(x.z, f[4], f[5]);
-                        k8_f16x4<E4M3>(x.w, f[6], f[7]);
-                        // K: [k tile of 64 dims][key group][8 dims][key], V: [key group][8 dims][key], 16 bytes each
-                        const uint32_t p = side == 0 ? out + c4 * 8192 + kg * 1024 + c_lo * 256 + key_lo * 16
-                                                     : out + M::f16_side + kg * (D * 16) + chunk * 256 + key_lo * 16;
-                        kt_sts(p, f[0], f[1], f[2], f[3]);
-                        kt_sts(p + 128, f[4], f[5], f[6], f[7]);
-                    }
-            };
-            if (beyond >= K8_PAGE) convert(std::false_type{});
-            else convert(std::true_type{});
-            if (threadIdx.x - 256 < 9) scales(KT_RAW + kv)[threadIdx.x - 256] = scales(st)[threadIdx.x - 256];
+                for (int u0 = 0; u0 < UNITS / 4; ++u0)
+                    if (((u0 & 1) * 4 + (warp - 8)) * 8 + key_lo >= beyond) x[u0] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int u0 = 0; u0 < UNITS / 4; ++u0) {
+                const int kg = (u0 & 1) * 4 + (warp - 8), c4 = u0 >> 1;
+                uint32_t f[8];
+                k8_f16x4<E4M3>(x[u0].x, f[0], f[1]);
+                k8_f16x4<E4M3>(x[u0].y, f[2], f[3]);
+                k8_f16x4<E4M3>(x[u0].z, f[4], f[5]);
+                k8_f16x4<E4M3>(x[u0].w, f[6], f[7]);
+                // K: [k tile of 64 dims][key group][8 dims][key], V: [key group][8 dims][key], 16 bytes each
+                const uint32_t p = out + key_lo * 16 + (side == 0 ? c4 * 8192 + kg * 1024 + c_lo * 256 : kg * (D * 16) + (c4 * 4 + c_lo) * 256);
+                kt_sts(p, f[0], f[1], f[2], f[3]);
+                kt_sts(p + 128, f[4], f[5], f[6], f[7]);
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            kt_arrive(bar + KT_KV_FULL + kv);
-            kt_arrive(bar + KT_RAW_EMPTY + st);
+            kt_arrive(bar + (side == 0 ? KT_K_FULL : KT_V_FULL) + (j & 1));
+        };
+        bool ok = true;
+        for (int i = 0; i <= n && n > 0 && ok; ++i) {
+            if (i < n) {                                                    // K of page i
+                ok = kt_wait(bar + KT_RAW_FULL + i % KT_RAW, i / KT_RAW) && (i < 2 || kt_wait(bar + KT_K_EMPTY + (i & 1), i / 2 - 1));
+                if (!ok) break;
+                if (warp == 8) {
+                    if (lane < 9) scales(KT_RAW + (i & 3))[lane] = scales(i % KT_RAW)[lane];
+                    __syncwarp();
+                    if (lane == 0) kt_arrive(bar + KT_SC + (i & 3));
+                }
+                convert(0, i);
+            }
+            if (i > 0) {                                                    // V of the page before
+                const int j = i - 1;
+                ok = j < 2 || kt_wait(bar + KT_V_EMPTY + (j & 1), j / 2 - 1);
+                if (!ok) break;
+                convert(1, j);
+                kt_arrive(bar + KT_RAW_EMPTY + j % KT_RAW);
+            }
         }
+        if (!ok && lane == 0) *s_fail = 1;
     } else {
         // ---- softmax: a thread a row
         const int w = warp >> 2, r = (warp & 3) * 32 + lane, rr = r0 + w * 128 + r;
@@ -264,12 +287,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv8_attend_tile(K8AttendArgs 
         const int mine = w == 0 ? nt[0] : nt[1];
         bool ok = true;
         for (int j = 0; j < mine && ok; ++j) {
-            ok = kt_wait(bar + KT_KV_FULL + (j & 1), j >> 1) && kt_wait(bar + KT_S + w * 2 + (j & 1), j >> 1);
+            ok = kt_wait(bar + KT_SC + (j & 3), j >> 2) && kt_wait(bar + KT_S + w * 2 + (j & 1), j >> 1);
             if (!ok) break;
             tc_fence_after();
             float sv[K8_PAGE];
             tc_ld_wait<K8_PAGE>(tm_s + (j & 1) * K8_PAGE, sv);
-            const float * sc = scales(KT_RAW + (j & 1));
+            const float * sc = scales(KT_RAW + (j & 3));
             const int kb = (t0 + j) * K8_PAGE;
             const bool none = reinterpret_cast<const int *>(sc)[8] != 0;
             const bool whole = !none && kb >= all_lo && kb + K8_PAGE <= all_hi;
