@@ -139,6 +139,7 @@ struct K8Plan { int kind, nt, tiles, ctas, part_rows; int64_t line_bytes, part_b
 constexpr int SMS = 148, NW = 4;
 bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     const int64_t R = (int64_t) p.max_q * (p.n_heads / c.n_kv_heads);
+    if (R > 0x7fffff00) return false;
     const bool tile = R > 64 && c.head_dim <= 128;
     o->nt = R <= 8 ? 1 : (R <= 16 || c.head_dim == 256 ? 2 : 4);
     const int per = tile ? KT_ROWS : 8 * o->nt;

@@ -49,6 +49,15 @@ _ROPE = struct.Struct("8if4x6Q8q")
 _ATTEND = struct.Struct("5Q4q4if4x3QqQq")
 assert _ROPE.size == C.sizeof(RopeArgs) and _ATTEND.size == C.sizeof(Kv8Attend)
 
+
+
+def _pack(fmt, *args):
+    try:
+        return fmt.pack(*args)
+    except struct.error as e:
+        raise ValueError(f"an argument is out of range: {e}") from None
+
+
 _torch = _L = None
 _types: dict = {}
 
@@ -161,7 +170,7 @@ def rope(q, k, positions, freq, *, layout: str = "half", factor: float = 1.0, q_
             kr, kd, _ = k.stride()
             kor, kod, _ = k_out.stride()
     if T:
-        _check(L.qtts_op_rope(_ROPE.pack(dev, _types[ty], T, heads, kh, dim, 2 * freq.shape[0], layout == "interleaved", factor, pos, freq.data_ptr(),
+        _check(L.qtts_op_rope(_pack(_ROPE, dev, _types[ty], T, heads, kh, dim, 2 * freq.shape[0], layout == "interleaved", factor, pos, freq.data_ptr(),
                                          q.data_ptr(), kp, q_out.data_ptr(), kop, qr, qh, kr, kd, qor, qoh, kor, kod), _stream(dev)))
     return q_out, k_out
 
@@ -325,11 +334,11 @@ class KvCache8:
         orow, oh, _ = out.stride()
         args = (tp, _int32(lens, self.seqs, self._dev, "lens"), cu_p or 0, q.data_ptr(), out.data_ptr(), qr, qh, orow, oh, T, most, heads, window, scale,
                 0 if lse is None else lse.data_ptr(), wi, wo, ws)
-        a = _ATTEND.pack(*args, 0, 0)
+        a = _pack(_ATTEND, *args, 0, 0)
         n = _L.qtts_kv8_attend_ws(c, a)
         if n > 0:
             space = _torch.empty(n, dtype=_torch.uint8, device=self.device)   # the stream's (or the graph's) own
-            a = _ATTEND.pack(*args, space.data_ptr(), n)
+            a = _pack(_ATTEND, *args, space.data_ptr(), n)
         _check(_L.qtts_op_kv8_attend(c, a, _stream(self._dev)))
         return out, lse
 

@@ -541,7 +541,8 @@ def test_refusals(kv8):
         lambda: c.append(x, x, t, n.cpu()), lambda: c.append(x, x, t, n, cu), lambda: c.append(x, x, t, n, cu[:2], 1), lambda: c.append(x, x, t, n, cu, -1),
         lambda: c.append(x.transpose(1, 2), x.transpose(1, 2), t, n), lambda: c.append(x, x, t.t(), n), lambda: c.append(x, x, t[:, :0].contiguous(), n),
         lambda: c.read(t, None, cu, 2, 1, torch.float64), lambda: c.read(t, n.long(), cu, 2, 1), lambda: c.read(t, None, cu, -1, 1), lambda: c.read(t, None, None, 3, 1),
-        lambda: c.attend(x[:, :1], t, n, scale=1.0), lambda: c.attend(x, t, n, cu, scale=1.0), lambda: c.attend(x, t, n, scale=1.0, window=-1),
+        lambda: c.attend(x[:, :1], t, n, scale=1.0), lambda: c.attend(x, t, n, cu, scale=1.0), lambda: c.attend(x, t, n, scale=1.0, window=-1), lambda: c.attend(x, t, n, scale=1.0, window=2 ** 40), lambda: c.attend(x, t, n, scale=-1.0),
+        lambda: c.attend(x, t, n, cu, 2 ** 31 - 1, scale=1.0),
         lambda: c.attend(x, t, n, scale=1.0, weight=w[..., :127].contiguous()), lambda: c.attend(x, t, n, scale=1.0, weight_out=w),
         lambda: c.attend(x, t, n, scale=1.0, weight=w.half()), lambda: c.attend(x, t, n, scale=1.0, out=x[:1]), lambda: c.attend(x[:, :0], t, n, scale=1.0),
         lambda: c.evict(t, n, t.clone(), w, 24), lambda: c.evict(t, n, t.clone(), w, 0), lambda: c.evict(t, n, t.clone(), w, 144), lambda: c.evict(t, n, t, w, 16),
