@@ -176,8 +176,11 @@ __device__ __forceinline__ float k8_load_q(K8Q<T, D> & q, const T * row, int lan
 // scale passes `unit` more than 8 times: most blocks need a vote and no reduction over
 // lanes.  A weight times its block's V scale over `unit`, at most 2^15, is rounded to
 // F16 for the product with V: half a step is 2^-12 relative, independent from key to
-// key and under the output's own rounding, or 2^-33 of the largest weight times the
-// largest V scale.  The sum of the weights is taken before that, in F32.
+// key, or 2^-33 of the largest weight times the largest V scale.  That is well under
+// the rounding of a BF16 output; for an F16 output, where it is as large (1.45 times the
+// plain form's error), the rest of the weight takes a second product with up to 8 rows
+// (the plain form's error, no time: 57.8 us against 59 at 32 sequences of 4,400).  The sum
+// of the weights is taken before that, in F32.
 constexpr float K8_LIFT = 8.0f, K8_SLACK = 4.0f, K8_UNIT_SLACK = 8.0f, K8_UNIT_MIN = 7.8886090522101181e-31f;   // 2^-100
 template <int D, int NT> struct K8State {
     float m[NT][2], l[NT][2], o[NT][D / 16][4];   // rows 8 nt + 2t, + 1
@@ -199,6 +202,7 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
                                           const K8AttendArgs & a, const int32_t * table, int h, int first, int last, int step, int all_lo, int all_hi,
                                           int any_hi, const K8Maps & maps, const K8Ring & R, uint32_t & phase, int lane) {
     constexpr int S = K8_SLOTS<D, NT>, U = K8_U<D, NT>, KEYS = U * K8_BLOCK, SPP = K8_PAGE / KEYS;
+    constexpr bool LOW = Row16<T>::inf == 0x7c00u && NT == 1;   // F16 rows: the weights' low halves too
     using Slot = K8Slot<D, U>;
     // a lane's places in a block: K chunk t of key kr (chunk 4 + t: ^ 64 bytes), V chunk g of keys 2t and vr
     const int g = lane >> 2, t = lane & 3, kr = k8_key(g), vr = k8_key(2 * t + 1);
@@ -320,6 +324,7 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
                 }
                 const float inv = __fdividef(1.0f, st.unit);
                 uint32_t p[U][NT][2];
+                [[maybe_unused]] uint32_t p_lo[U][NT][2];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const float rv = vs[u] * inv;
@@ -334,8 +339,16 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
                             st.l[nt][i & 1] += hidden ? 0.0f : x;
                             e[i] = hidden ? 0.0f : x * rv;
                         }
-                        p[u][nt][0] = k8_transpose(k8_pack(e[0], e[1]));   // rows of the transpose: keys 2t, 2t + 1 in MMA order
-                        p[u][nt][1] = k8_transpose(k8_pack(e[2], e[3]));
+                        // rows of the transpose: keys 2t, 2t + 1 in MMA order
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t hi = k8_pack(e[2 * i], e[2 * i + 1]);
+                            p[u][nt][i] = k8_transpose(hi);
+                            if constexpr (LOW) {
+                                const float2 f = k8_f32x2(hi);
+                                p_lo[u][nt][i] = k8_transpose(k8_pack(e[2 * i] - f.x, e[2 * i + 1] - f.y));
+                            }
+                        }
                     }
                 }
 #pragma unroll
@@ -373,7 +386,10 @@ __device__ __forceinline__ void k8_blocks(K8State<D, NT> & st, const K8Q<T, D> (
                             for (int o = 0; o < 2; ++o)
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt)
+                                    {
                                     k8_mma(st.o[nt][c * 8 + 2 * w + o], a0[o], a1[o], a2[o], a3[o], p[u][nt][0], p[u][nt][1]);
+                                    if constexpr (LOW) k8_mma(st.o[nt][c * 8 + 2 * w + o], a0[o], a1[o], a2[o], a3[o], p_lo[u][nt][0], p_lo[u][nt][1]);
+                                }
                         }
                     }
                 }
