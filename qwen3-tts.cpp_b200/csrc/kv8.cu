@@ -131,16 +131,20 @@ template <class F> void by_cache(const qtts_kv8 & c, F f) {
     else by_code(__nv_bfloat16{});
 }
 
-// How an attention call runs.  Up to 64 rows of a (sequence, kv head) come in tiles of
-// 8 nt; one CTA takes a tile's whole range, or, where that is more than 8 pages, the
-// ranges are split evenly over the GPU.  More rows come in tiles of 256 on tcgen05.
+// How an attention call runs.  Few rows of a (sequence, kv head) come in tiles of 8 nt;
+// one CTA takes a tile's whole range, or, where that is more than 8 pages, the ranges
+// are split evenly over the GPU.  Many rows come in tiles of 256 on tcgen05, one CTA each.
+// Where they meet, at 2,000 keys, 8 kv heads, dim 128 (us, split / tile): 32 rows, 1, 8 and
+// 32 sequences 31 / 51, 47 / 52, 102 / 103; 64 rows 33 / 51, 66 / 53, 182 / 105.  So from
+// 33 rows on the tiles are taken where there are CTAs for half of the SMs, and from 65 on
+// always (the split kernel would read the cache once for each 32 rows).
 enum : int { PLAN_WHOLE, PLAN_SPLIT, PLAN_TILE };
 struct K8Plan { int kind, nt, tiles, ctas, part_rows; int64_t line_bytes, part_bytes; unsigned grid; };   // workspace: line, parts, lse
 constexpr int SMS = 148, NW = 4;
 bool attend_plan(const qtts_kv8 & c, const qtts_kv8_attend & p, K8Plan * o) {
     const int64_t R = (int64_t) p.max_q * (p.n_heads / c.n_kv_heads);
     if (R > 0x7fffff00) return false;
-    const bool tile = R > 64 && c.head_dim <= 128;
+    const bool tile = c.head_dim <= 128 && (R > 64 || (R > 32 && (int64_t) c.n_seqs * c.n_kv_heads >= 64));
     o->nt = R <= 8 ? 1 : (R <= 16 || c.head_dim == 256 ? 2 : 4);
     const int per = tile ? KT_ROWS : 8 * o->nt;
     const int64_t tiles = (R + per - 1) / per, items = tiles * c.n_kv_heads * c.n_seqs;

@@ -21,8 +21,9 @@
 // scheduler for the scores' arithmetic and the conversion.  Measured: 0.84 ms for 2,048
 // tokens of 32 heads over 16,384 keys (613 TFLOP/s, 36% of the measured GEMM rate), some
 // 3,000 cycles a page: the hand-offs softmax -> MMA -> softmax are what is left (without
-// conversion and exponentials they took 70% of an earlier version's time).  More than 64
-// rows come here; below, the padding to 128 rows costs more than the tensor core gives.
+// conversion and exponentials they took 70% of an earlier version's time).  P
+// in tensor memory over the scores (its A operand) measured 0.91 ms: the scores two pages
+// on then have to wait for the product.
 #pragma once
 #include "kv8_attend.cuh"
 #include "tcgen05.cuh"

@@ -297,7 +297,8 @@ def test_attend_windows(kv8, window):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("D,H,heads,n", [(128, 2, 4, [1, 15, 7, 17, 0, 64, 3, 130, 90]), (64, 1, 5, [1, 1, 2, 3, 4, 3, 2, 1, 3]),
                                          (128, 1, 8, [1, 2, 2, 2, 2, 2, 2, 2, 2]), (256, 1, 2, [1, 15, 16, 17, 63, 64, 65, 1, 299]),
-                                         (64, 2, 6, [0, 0, 0, 0, 0, 0, 0, 130, 257])])
+                                         (64, 2, 6, [0, 0, 0, 0, 0, 0, 0, 130, 257]),
+                                         (64, 8, 16, [1, 15, 16, 17, 20, 20, 0, 3, 20]), (128, 8, 32, [0, 9, 10, 11, 12, 1, 16, 16, 15])])
 def test_attend_several_rows(kv8, code, dtype, D, H, heads, n):
     a = Both(kv8, len(LENS), H, D, code, dtype, cols=5, seed=7)
     a.append(LENS)
