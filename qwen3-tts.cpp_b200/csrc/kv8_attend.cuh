@@ -80,7 +80,7 @@ __device__ __forceinline__ uint32_t k8_transpose(uint32_t x) {   // an 8 x 8 mat
 }
 __device__ __forceinline__ int k8_key(int g) { return g ^ (g & 1) << 2; }   // the key of MMA row g
 
-struct K8Maps { CUtensorMap k, v; };             // the pools as [pages * kv heads * 64][D] bytes, boxes of k8_box rows x min(D, 128)
+struct K8Maps { CUtensorMap k, v; };             // the pools as [pages * kv heads * 64][D] bytes, boxes of a step's rows x min(D, 128)
 
 // A slot of a warp's ring in shared memory: the K and the V rows of U blocks (D = 256: in
 // two halves of 128 dims), swizzled.  Beside the ring: the page's scales and a barrier

@@ -16,8 +16,8 @@
 // rescaled.  Codes are scaled after the products in F32: the scores per 16 keys, V through
 // the weights.
 //
-// Bound per 64 keys and 256 rows at D = 128: 1,020 cycles of MMA (8,192 F16 FMA a cycle
-// and SM at the measured peak), 1,024 of exponentials (16 a cycle), some 1,000 issue slots a
+// Bound per 64 keys and 256 rows at D = 128: 1,020 cycles of MMA (4,108 F16 FMA a cycle
+// and SM at the nominal peak), 1,024 of exponentials (16 a cycle), some 1,000 issue slots a
 // scheduler for the scores' arithmetic and the conversion.  Measured: 0.84 ms for 2,048
 // tokens of 32 heads over 16,384 keys (613 TFLOP/s, 36% of the measured GEMM rate), some
 // 3,000 cycles a page: the hand-offs softmax -> MMA -> softmax are what is left (without
